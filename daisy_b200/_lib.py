@@ -89,7 +89,17 @@ SIGNATURES = {
     "daisy_b200_kda_short_conv": (_i, [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i, _i, _i, _i, _u, _vp]),
     "daisy_b200_kda_out_norm": (_i, [_vp, _i, _vp, _vp, _i, _vp, _vp, _i64, _i, _f, _i, _vp]),
     "daisy_b200_selftest_umma": (_i, [_vp] * 3 + [_i, _i, _vp, _vp]),
+    "daisy_b200_paged_append": (_i, [_vp] * 4 + [_i64] * 9 + [_vp] * 5 + [_i] + [_vp] + [_i64] * 3 + [_vp] + [_i] * 4 + [_f, _u, _vp, _vp]),
+    "daisy_b200_paged_decode_workspace_bytes": (_sz, [_i] * 4),
+    "daisy_b200_paged_decode_step": (_i, [_vp] * 4 + [_i64] * 6 + [_vp, _i, _vp, _vp, _i] + [_vp, _i64, _i64] + [_vp, _i64, _i64, _vp] +
+                                     [_i] * 2 + [_f, _f, _u, _vp, _sz, _vp, _vp]),
 }
+
+
+class Pages(C.Structure):
+    """``daisy_b200_pages``: the pool of a paged cache and its table."""
+    _fields_ = [("k", _vp), ("v", _vp), ("p_sb", _i64), ("p_sh", _i64), ("p_sr", _i64), ("table", _vp), ("table_sb", _i64),
+                ("n_pages", _i), ("H", _i), ("page", _i), ("width", _i), ("n_seq", _i)]
 
 _lib = None
 

@@ -1,0 +1,508 @@
+// One new token of every sequence against a paged cache: the work of a batch of uneven lengths dealt out in equal shares, one launch.
+//
+// Bound by HBM: 512 bytes for every cached row and key head, read once for all query heads of the group.  The cached rows
+// of all (sequence, key head) pairs lie end to end in tiles of 16; every CTA takes an equal run of tiles, whatever sequences it
+// cuts, so neither uneven lengths nor a wide block table leaves an SM idle (the host knows no lengths).  A pair that
+// several CTAs share is joined by the last of them, from partial sums in a fixed order: the same bits every run.  That last one,
+// or the only one, also prepares the token's own row, adds it and stores it.
+//
+// A warp takes a tile straight from memory into the operands of mma.m16n8k16 (keys or channels are the 16, query heads the 8; every lane
+// loads whole 16-byte pieces, the order of channels in a product is free): scores S^T = K Q^T, then O^T += V^T P^T.  On CUDA cores
+// the same work is 22 instructions for 16 bytes and lane, a third of the SM's issue slots for one query head and over all of them for
+// four.  Queries and weights go in as sums of two 16-bit values (two products each): scores and weights keep 16 bits and more.
+#include "paged.cuh"
+
+namespace daisy {
+
+constexpr int PD_WARPS = 4;
+constexpr int PD_TILE = 16;
+constexpr float PD_NEG = -1.0e30f;
+
+struct PagedDecodeParams {
+  PagedCache c;
+  const __nv_bfloat16 *q, *k, *v, *ve;
+  int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh, ve_sb, ve_sh, o_sb, o_sh;
+  __nv_bfloat16* out;
+  const int* lens;
+  const float *cos, *sin, *ve_gate;
+  int window, table_rows, Hq, G;     // G query heads of one key head; they come in n_grp groups of at most 8 NT
+  int n_grp;
+  float qscale, eps;
+  unsigned flags;
+  int* status;
+  float* part;                       // [2 grid][8 NT][PD_PART]: 128 sums, reference, denominator
+  int* tickets;                      // [n_seq H n_grp], zero between calls
+};
+constexpr int PD_PART = 132;
+constexpr __host__ __device__ int pd_ctas(int cols) { return cols == 8 ? 3 : 2; }              // CTAs a SM, by registers
+
+// Where a sequence stands: its cached length, or -1 if it is idle or cannot have the position; rows lo .. len-1 are seen.
+struct SeqRange { int len, lo, tile0, tiles; };
+__device__ __forceinline__ SeqRange seq_range(const PagedDecodeParams& p, int b) {
+  SeqRange r;
+  r.len = p.lens[b];
+  const bool bad = r.len >= p.c.capacity() || ((p.flags & DAISY_ROPE) && r.len >= p.table_rows);
+  if (bad && p.status) p.status[0] = DAISY_EINVAL;
+  if (r.len < 0 || bad) r.len = -1;
+  r.lo = p.window > 0 && r.len > p.window - 1 ? r.len - (p.window - 1) : 0;
+  r.tile0 = r.lo / PD_TILE;
+  r.tiles = r.len <= r.lo ? 1 : (r.len + PD_TILE - 1) / PD_TILE - r.tile0;      // one without rows: the token alone
+  return r;
+}
+
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+// Four channels 4 lane .. 4 lane + 3 of a row, normalised and rotated by the whole warp.
+__device__ __forceinline__ void row_of_warp(const __nv_bfloat16* src, bool norm, bool rope, float eps, const float* cos_row, const float* sin_row,
+                                            int lane, float (&x)[4]) {
+  const uint2 u = *reinterpret_cast<const uint2*>(src + 4 * lane);
+  x[0] = bf16_lo(u.x); x[1] = bf16_hi(u.x); x[2] = bf16_lo(u.y); x[3] = bf16_hi(u.y);
+  if (norm) {
+    const float r = rsqrtf(warp_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]) * (1.0f / DAISY_HEAD_DIM) + eps);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] *= r;
+  }
+  if (rope) {
+    const float4 c = *reinterpret_cast<const float4*>(cos_row + 4 * (lane & 15)), s = *reinterpret_cast<const float4*>(sin_row + 4 * (lane & 15));
+    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+    const float sgn = lane < 16 ? 1.f : -1.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float other = __shfl_xor_sync(0xffffffffu, x[e], 16);
+      x[e] = x[e] * cc[e] + sgn * other * ss[e];
+    }
+  }
+}
+
+// Sum over all sequences of their tiles; with `want` >= 0 also the sequence that holds tile `want` of the batch (tiles of one head)
+// and the tiles in front of it.  The whole block calls it.
+struct Found { int64_t total; int b; int64_t before; };
+__device__ __forceinline__ Found scan_tiles(const PagedDecodeParams& p, int64_t want, int64_t* sm) {
+  Found f{0, -1, 0};
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int b0 = 0; b0 < p.c.n_seq; b0 += 32 * PD_WARPS) {
+    const int b = b0 + threadIdx.x;
+    const int64_t t = b < p.c.n_seq ? seq_range(p, b).tiles : 0;
+    int64_t x = t;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sm[warp] = x;
+    if (threadIdx.x == 0) sm[PD_WARPS] = -1;
+    __syncthreads();
+    int64_t base = f.total, sum = 0;
+    for (int w = 0; w < PD_WARPS; ++w) { if (w < warp) base += sm[w]; sum += sm[w]; }
+    if (want >= 0 && t > 0 && base + x - t <= want && want < base + x) { sm[PD_WARPS] = b; sm[PD_WARPS + 1] = base + x - t; }
+    __syncthreads();
+    if (want >= 0 && sm[PD_WARPS] >= 0) { f.b = (int)sm[PD_WARPS]; f.before = sm[PD_WARPS + 1]; return f; }
+    f.total += sum;
+  }
+  return f;
+}
+
+template <int NT, bool F16>
+__global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_kernel(const PagedDecodeParams p) {
+  constexpr int NQ = 8 * NT;                                         // query heads of a pass, the last ones maybe absent
+  __shared__ int64_t sm_scan[PD_WARPS + 2];
+  __shared__ __align__(16) float sm_acc[PD_WARPS][NQ][DAISY_HEAD_DIM];
+  __shared__ float sm_m[PD_WARPS][NQ], sm_l[PD_WARPS][NQ];
+  __shared__ float sm_self[NQ];
+  __shared__ __align__(16) float sm_v[DAISY_HEAD_DIM];
+  __shared__ int sm_last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int HH = p.c.H * p.n_grp;                                    // pairs a sequence
+  grid_dep_launch();
+  grid_dep_wait();
+
+  const int64_t total = scan_tiles(p, -1, sm_scan).total * HH;
+  int64_t share = (total + gridDim.x - 1) / gridDim.x;
+  share = (share + PD_WARPS - 1) / PD_WARPS * PD_WARPS;
+  int64_t t = (int64_t)blockIdx.x * share;
+  const int64_t t_end = min(t + share, total);
+  if (t >= t_end) return;
+  const Found f = scan_tiles(p, t / HH, sm_scan);                    // pairs are (sequence, head)-major: head h of b begins at before HH + h tiles
+  int b = f.b;
+  if (b < 0) return;
+  int64_t b_at = f.before * HH;
+  SeqRange r = seq_range(p, b);
+
+  while (t < t_end) {
+    while (t >= b_at + (int64_t)r.tiles * HH) {
+      if (b + 1 >= p.c.n_seq) return;                                // lengths that changed under the call
+      b_at += (int64_t)r.tiles * HH;
+      r = seq_range(p, ++b);
+    }
+    const int hh = (int)((t - b_at) / r.tiles), h = hh / p.n_grp, grp = hh % p.n_grp;
+    const int64_t u_at = b_at + (int64_t)hh * r.tiles;               // this pair's tiles: u_at .. u_end - 1
+    const int64_t u_end = u_at + r.tiles, s_end = min(u_end, t_end);
+    const int q_h0 = h * p.G + grp * NQ, n_q = min(NQ, p.G - grp * NQ);
+    const float *cos_row = p.cos + (int64_t)max(r.len, 0) * 64, *sin_row = p.sin + (int64_t)max(r.len, 0) * 64;
+
+    // ---------------------------------------------------------------- the queries as B operands: lane (g, c) holds head 8 n + g, channels
+    // 32 j + 8 c .. + 7 for j = 0..3; element pair i of piece j goes to k step 2 j + i / 2
+    uint32_t qh[NT][4][4], ql[NT][4][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float x[4][8];
+      const bool live = 8 * n + g < n_q;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint4 u = live ? ld_cg16(p.q + b * p.q_sb + (q_h0 + 8 * n + g) * p.q_sh + 32 * j + 8 * c) : make_uint4(0, 0, 0, 0);
+        unpack8(u, x[j]);
+      }
+      float mul = p.qscale;
+      if (p.flags & DAISY_NORM_Q) {
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss = fmaf(x[j][e], x[j][e], ss);
+        ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+        ss += __shfl_xor_sync(0xffffffffu, ss, 2);
+        mul *= rsqrtf(ss * (1.0f / DAISY_HEAD_DIM) + p.eps);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float cs = 1.f, sn = 0.f;
+          if (p.flags & DAISY_ROPE) { cs = cos_row[32 * j + 8 * c + e]; sn = sin_row[32 * j + 8 * c + e]; }
+          const float a = x[j][e] * mul, d = x[j + 2][e] * mul;
+          x[j][e] = a * cs + d * sn;
+          x[j + 2][e] = d * cs - a * sn;
+        }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          qh[n][j][i] = pack16<F16>(x[j][2 * i], x[j][2 * i + 1]);
+          const float2 back = unpack16<F16>(qh[n][j][i]);
+          ql[n][j][i] = pack16<F16>(x[j][2 * i] - back.x, x[j][2 * i + 1] - back.y);
+        }
+    }
+
+    float acc[NT][8][4];                                             // channels 8 g + e (elements 0, 1) and 64 + 8 g + e of heads 2 c, 2 c + 1
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[n][e][0] = acc[n][e][1] = acc[n][e][2] = acc[n][e][3] = 0.f;
+      m[n][0] = m[n][1] = PD_NEG;
+      l[n][0] = l[n][1] = 0.f;
+    }
+
+    const int* table = p.c.table + b * p.c.table_sb;
+    const int first = r.tile0 + (int)(t - u_at), last = r.tile0 + (int)(s_end - u_at);    // tiles of the sequence
+    auto page_of = [&](int tile) -> int {                            // a row outside the pool is taken from page 0
+      int pg = tile < last && r.len > r.lo ? table[(tile * PD_TILE) >> p.c.lg] : 0;
+      if ((unsigned)pg >= (unsigned)p.c.n_pages) {
+        if (p.status) p.status[0] = DAISY_EINVAL;
+        pg = 0;
+      }
+      return pg;
+    };
+    int pg = page_of(first + warp);
+    for (int tile = first + warp; tile < last; tile += PD_WARPS) {
+      const int row0 = tile * PD_TILE;
+      const char *kb = p.c.k + p.c.at(pg, h, row0) + 16 * c, *vb = p.c.v + p.c.at(pg, h, row0) + 16 * g;
+      const int64_t sr = 2 * p.c.p_sr;
+      const bool whole = row0 >= r.lo && row0 + PD_TILE <= r.len;
+      uint4 kk[2][4], vv[4][2];
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) kk[i][j] = ld_stream16(kb + (g + 8 * i) * sr + 64 * j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) vv[i][j] = ld_stream16(vb + (2 * c + (i & 1) + 8 * (i >> 1)) * sr + 128 * j);
+      } else {                                                       // rows that nobody sees may hold anything: they count as zeros
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = g + 8 * i;
+          const bool in = row0 + row >= r.lo && row0 + row < r.len;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) kk[i][j] = in ? ld_stream16(kb + row * sr + 64 * j) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = 2 * c + (i & 1) + 8 * (i >> 1);
+          const bool in = row0 + row >= r.lo && row0 + row < r.len;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) vv[i][j] = in ? ld_stream16(vb + row * sr + 128 * j) : make_uint4(0, 0, 0, 0);
+        }
+      }
+      pg = page_of(tile + PD_WARPS);
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t k0[4] = {kk[0][j].x, kk[0][j].y, kk[0][j].z, kk[0][j].w}, k1[4] = {kk[1][j].x, kk[1][j].y, kk[1][j].z, kk[1][j].w};
+#pragma unroll
+        for (int i = 0; i < 4; i += 2)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma16816<F16>(s[n], k0[i], k1[i], k0[i + 1], k1[i + 1], qh[n][j][i], qh[n][j][i + 1]);
+            mma16816<F16>(s[n], k0[i], k1[i], k0[i + 1], k1[i + 1], ql[n][j][i], ql[n][j][i + 1]);
+          }
+      }
+      if (!whole) {
+        const bool in0 = row0 + g >= r.lo && row0 + g < r.len, in1 = row0 + g + 8 >= r.lo && row0 + g + 8 < r.len;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (!in0) s[n][0] = s[n][1] = -INFINITY;
+          if (!in1) s[n][2] = s[n][3] = -INFINITY;
+        }
+      }
+      uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float t0 = fmaxf(s[n][0], s[n][2]), t1 = fmaxf(s[n][1], s[n][3]);
+        // the reference follows the maximum only when that has grown by over 2^8: sums stay far inside their range
+        if (__any_sync(0xffffffffu, t0 > m[n][0] + 8.f || t1 > m[n][1] + 8.f)) {
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
+            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
+          }
+          t0 = fmaxf(t0, m[n][0]); t1 = fmaxf(t1, m[n][1]);
+          const float a0 = fast_exp2(m[n][0] - t0), a1 = fast_exp2(m[n][1] - t1);
+          m[n][0] = t0; m[n][1] = t1;
+          l[n][0] *= a0; l[n][1] *= a1;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) { acc[n][e][0] *= a0; acc[n][e][1] *= a1; acc[n][e][2] *= a0; acc[n][e][3] *= a1; }
+        }
+        const float w0 = fast_exp2(s[n][0] - m[n][0]), w1 = fast_exp2(s[n][1] - m[n][1]);
+        const float w2 = fast_exp2(s[n][2] - m[n][0]), w3 = fast_exp2(s[n][3] - m[n][1]);
+        l[n][0] += w0 + w2; l[n][1] += w1 + w3;
+        const uint32_t h0 = pack16<F16>(w0, w1), h1 = pack16<F16>(w2, w3);
+        const float2 b0 = unpack16<F16>(h0), b1 = unpack16<F16>(h1);
+        ph[n][0] = transpose8x8(h0); ph[n][1] = transpose8x8(h1);
+        pl[n][0] = transpose8x8(pack16<F16>(w0 - b0.x, w1 - b0.y)); pl[n][1] = transpose8x8(pack16<F16>(w2 - b1.x, w3 - b1.y));
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        uint32_t a[4];                                               // channels 8 g + e, 64 + 8 g + e of keys 2 c, 2 c + 1 | 2 c + 8, 2 c + 9
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 lo4 = vv[i & 2][i & 1], hi4 = vv[(i & 2) + 1][i & 1];
+          const uint32_t lo = e < 2 ? lo4.x : e < 4 ? lo4.y : e < 6 ? lo4.z : lo4.w, hi = e < 2 ? hi4.x : e < 4 ? hi4.y : e < 6 ? hi4.z : hi4.w;
+          a[i] = __byte_perm(lo, hi, (e & 1) ? 0x7632 : 0x5410);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma16816<F16>(acc[n][e], a[0], a[1], a[2], a[3], ph[n][0], ph[n][1]);
+          mma16816<F16>(acc[n][e], a[0], a[1], a[2], a[3], pl[n][0], pl[n][1]);
+        }
+      }
+    }
+
+    // ---------------------------------------------------------------- the four warps' sums
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x = l[n][i];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        const int col = 8 * n + 2 * c + i;
+        if (col < n_q) {
+          if (g == 0) { sm_m[warp][col] = m[n][i]; sm_l[warp][col] = x; }
+          float* dst = &sm_acc[warp][col][8 * g];
+          *reinterpret_cast<float4*>(dst) = make_float4(acc[n][0][i], acc[n][1][i], acc[n][2][i], acc[n][3][i]);
+          *reinterpret_cast<float4*>(dst + 4) = make_float4(acc[n][4][i], acc[n][5][i], acc[n][6][i], acc[n][7][i]);
+          *reinterpret_cast<float4*>(dst + 64) = make_float4(acc[n][0][2 + i], acc[n][1][2 + i], acc[n][2][2 + i], acc[n][3][2 + i]);
+          *reinterpret_cast<float4*>(dst + 68) = make_float4(acc[n][4][2 + i], acc[n][5][2 + i], acc[n][6][2 + i], acc[n][7][2 + i]);
+        }
+      }
+    __syncthreads();
+    const int d = threadIdx.x;
+    const bool alone = u_at >= (int64_t)blockIdx.x * share && u_end <= t_end;
+    // this CTA's sums of head `col`: numerator of channel d, reference, denominator
+    auto mine = [&](int col, float& num, float& ref, float& den) {
+      ref = fmaxf(fmaxf(sm_m[0][col], sm_m[1][col]), fmaxf(sm_m[2][col], sm_m[3][col]));
+      num = den = 0.f;
+#pragma unroll
+      for (int w = 0; w < PD_WARPS; ++w) {
+        const float s = fast_exp2(sm_m[w][col] - ref);
+        num = fmaf(s, sm_acc[w][col][d], num);
+        den = fmaf(s, sm_l[w][col], den);
+      }
+    };
+    bool finish = alone;
+    const int64_t c0 = u_at / share, c1 = (u_end - 1) / share;        // the CTAs that share this pair
+    if (!alone) {
+      float* dst = p.part + ((int64_t)blockIdx.x * 2 + (blockIdx.x == c0 ? 1 : 0)) * NQ * PD_PART;
+      for (int col = 0; col < n_q; ++col) {
+        float num, ref, den;
+        mine(col, num, ref, den);
+        dst[col * PD_PART + d] = num;
+        if (d == 0) { dst[col * PD_PART + 128] = ref; dst[col * PD_PART + 129] = den; }
+      }
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        int* tk = p.tickets + ((int64_t)b * HH + hh);
+        const int drawn = atomicAdd(tk, 1);
+        sm_last = drawn == (int)(c1 - c0);
+        if (sm_last) *tk = 0;                                        // every other one has been drawn
+      }
+      __syncthreads();
+      finish = sm_last != 0;
+      if (finish) __threadfence();
+    }
+    if (finish) {
+      // ---------------------------------------------------------------- the token's own row
+      if (r.len >= 0) {
+        float kr[4], vr[4];
+        row_of_warp(p.k + b * p.k_sb + h * p.k_sh, p.flags & DAISY_NORM_K, p.flags & DAISY_ROPE, p.eps, cos_row, sin_row, lane, kr);
+        row_of_warp(p.v + b * p.v_sb + h * p.v_sh, p.flags & DAISY_NORM_V, false, p.eps, cos_row, sin_row, lane, vr);
+        if (p.ve) {
+          const float gate = 1.0f / (1.0f + __expf(-*p.ve_gate));
+          const uint2 u = *reinterpret_cast<const uint2*>(p.ve + b * p.ve_sb + h * p.ve_sh + 4 * lane);
+          const float e[4] = {bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y)};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vr[i] = gate * vr[i] + (1.0f - gate) * e[i];
+        }
+        const uint2 k16 = make_uint2(pack16<F16>(kr[0], kr[1]), pack16<F16>(kr[2], kr[3]));
+        const uint2 v16 = make_uint2(pack16<F16>(vr[0], vr[1]), pack16<F16>(vr[2], vr[3]));
+        const float2 ka = unpack16<F16>(k16.x), kc = unpack16<F16>(k16.y), va = unpack16<F16>(v16.x), vc = unpack16<F16>(v16.y);
+        for (int col = warp; col < n_q; col += PD_WARPS) {
+          float x[4];
+          row_of_warp(p.q + b * p.q_sb + (q_h0 + col) * p.q_sh, p.flags & DAISY_NORM_Q, p.flags & DAISY_ROPE, p.eps, cos_row, sin_row, lane, x);
+          const float s = warp_sum(x[0] * ka.x + x[1] * ka.y + x[2] * kc.x + x[3] * kc.y) * p.qscale;
+          if (lane == 0) sm_self[col] = s;
+        }
+        if (warp == 0) {
+          *reinterpret_cast<float4*>(&sm_v[4 * lane]) = make_float4(va.x, va.y, vc.x, vc.y);
+          if (grp == 0) {
+            const int new_pg = table[r.len >> p.c.lg];
+            if ((unsigned)new_pg < (unsigned)p.c.n_pages) {
+              const int64_t at = p.c.at(new_pg, h, r.len) + 8 * lane;
+              *reinterpret_cast<uint2*>(p.c.k + at) = k16;
+              *reinterpret_cast<uint2*>(p.c.v + at) = v16;
+            } else if (p.status && lane == 0) {
+              p.status[0] = DAISY_EINVAL;
+            }
+          }
+        }
+      }
+      __syncthreads();
+      for (int col = 0; col < n_q; ++col) {
+        float y = 0.f;
+        if (r.len >= 0) {
+          float num, ref, den;
+          if (alone) {
+            mine(col, num, ref, den);
+          } else {
+            ref = PD_NEG; num = den = 0.f;
+            for (int64_t cc = c0; cc <= c1; ++cc) {
+              const float* src = p.part + (cc * 2 + (cc == c0 ? 1 : 0)) * NQ * PD_PART + col * PD_PART;
+              const float n1 = __ldcg(src + d), r1 = __ldcg(src + 128), d1 = __ldcg(src + 129);
+              const float top = fmaxf(ref, r1), a = fast_exp2(ref - top), e = fast_exp2(r1 - top);
+              num = num * a + n1 * e;
+              den = den * a + d1 * e;
+              ref = top;
+            }
+          }
+          const float self = sm_self[col], top = fmaxf(ref, self), a = fast_exp2(ref - top), w = fast_exp2(self - top);
+          y = (num * a + w * sm_v[d]) / (den * a + w);
+        }
+        p.out[b * p.o_sb + (q_h0 + col) * p.o_sh + d] = __float2bfloat16_rn(y);
+      }
+    }
+    t = s_end;
+    if (t < t_end) __syncthreads();                                  // shared memory is used again
+  }
+}
+
+}  // namespace daisy
+
+using namespace daisy;
+
+// query heads a pass: 8, or 16 where a key head has more than 8
+static int decode_cols(int G) { return G > 8 ? 16 : 8; }
+// Partial sums of either form.  The tickets begin behind them whatever the sizes of a call are: calls of different sizes share a
+// workspace, and only tickets are ever written where another call's tickets lie.
+static size_t partials_bytes(int sms) {
+  constexpr size_t cols = pd_ctas(8) * 8 > pd_ctas(16) * 16 ? pd_ctas(8) * 8 : pd_ctas(16) * 16;
+  return (size_t)sms * 2 * cols * PD_PART * sizeof(float);
+}
+
+extern "C" size_t daisy_b200_paged_decode_workspace_bytes(int n_seq, int Hq, int H, int D) {
+  if (n_seq <= 0 || Hq <= 0 || H <= 0 || D != DAISY_HEAD_DIM || Hq % H) return 0;
+  int sms = daisy_host::sm_count_cached();
+  if (sms <= 0) sms = daisy_host::MAX_SMS;
+  const int nq = decode_cols(Hq / H), n_grp = (Hq / H + nq - 1) / nq;
+  return partials_bytes(sms) + ((size_t)n_seq * H * n_grp * sizeof(int) + 15) / 16 * 16;
+}
+
+extern "C" int daisy_b200_paged_decode_step(const daisy_b200_pages* cache, const void* q_new, const void* k_new, const void* v_new,
+                                            int64_t q_sb, int64_t q_sh, int64_t k_sb, int64_t k_sh, int64_t v_sb, int64_t v_sh,
+                                            const int32_t* lens, int window, const float* cos, const float* sin, int table_rows,
+                                            void* out, int64_t o_sb, int64_t o_sh,
+                                            const void* ve, int64_t ve_sb, int64_t ve_sh, const float* ve_gate_logit,
+                                            int Hq, int D, float scale, float eps, unsigned flags,
+                                            void* workspace, size_t workspace_bytes, int* status_word, void* stream) {
+  PagedDecodeParams p = {};
+  if (const int rc = daisy_host::paged_cache(cache, D, &p.c); rc != DAISY_OK) return rc;
+  if (!q_new || !k_new || !v_new || !lens || !out || !workspace || Hq <= 0 || Hq % cache->H) return DAISY_EINVAL;
+  if (flags & ~(DAISY_QKV_DEFAULT | DAISY_CACHE_FP16)) return DAISY_EINVAL;
+  if ((flags & DAISY_ROPE) && (!cos || !sin || table_rows <= 0)) return DAISY_EINVAL;
+  if (ve && (!ve_gate_logit || !(flags & DAISY_NORM_V))) return DAISY_EINVAL;
+  if (!daisy_aligned16(q_new) || !daisy_aligned16(k_new) || !daisy_aligned16(v_new) || !daisy_aligned16(ve) || !daisy_aligned16(workspace) ||
+      ((q_sb | q_sh | k_sb | k_sh | v_sb | v_sh) & 7) || (ve && ((ve_sb | ve_sh) & 7)) || (reinterpret_cast<uintptr_t>(lens) & 3) ||
+      (reinterpret_cast<uintptr_t>(out) & 1))
+    return DAISY_EALIGN;
+  if ((flags & DAISY_ROPE) && (!daisy_aligned16(cos) || !daisy_aligned16(sin))) return DAISY_EALIGN;
+  if (workspace_bytes < daisy_b200_paged_decode_workspace_bytes(cache->n_seq, Hq, cache->H, D)) return DAISY_EWORKSPACE;
+  const int sms = daisy_host::sm_count_cached();
+  if (sms <= 0) return DAISY_ENODEV;
+  p.G = Hq / cache->H; p.Hq = Hq;
+  const int nq = decode_cols(p.G);
+  p.n_grp = (p.G + nq - 1) / nq;
+  if ((int64_t)cache->n_seq * cache->H * p.n_grp >= (int64_t)1 << 31) return DAISY_EUNSUPPORTED;
+  p.q = (const __nv_bfloat16*)q_new; p.k = (const __nv_bfloat16*)k_new; p.v = (const __nv_bfloat16*)v_new; p.ve = (const __nv_bfloat16*)ve;
+  p.q_sb = q_sb; p.q_sh = q_sh; p.k_sb = k_sb; p.k_sh = k_sh; p.v_sb = v_sb; p.v_sh = v_sh; p.ve_sb = ve_sb; p.ve_sh = ve_sh;
+  p.o_sb = o_sb; p.o_sh = o_sh;
+  p.out = (__nv_bfloat16*)out;
+  p.lens = lens; p.cos = cos; p.sin = sin; p.ve_gate = ve_gate_logit;
+  p.window = window; p.table_rows = table_rows;
+  p.qscale = scale * 1.4426950408889634f;
+  p.eps = eps; p.flags = flags; p.status = status_word;
+  const unsigned grid = (unsigned)(sms * pd_ctas(nq));
+  p.part = (float*)workspace;
+  p.tickets = (int*)((char*)workspace + partials_bytes(sms));
+  const bool f16 = (flags & DAISY_CACHE_FP16) != 0;
+  cudaStream_t st = (cudaStream_t)stream;
+  auto go = [&](auto kernel) { return daisy_host::launch_dependent(kernel, dim3(grid), dim3(32 * PD_WARPS), 0, st, p); };
+  const cudaError_t e = nq == 8 ? (f16 ? go(paged_decode_kernel<1, true>) : go(paged_decode_kernel<1, false>))
+                                : (f16 ? go(paged_decode_kernel<2, true>) : go(paged_decode_kernel<2, false>));
+  if (e != cudaSuccess) { (void)cudaGetLastError(); return DAISY_ECUDA; }
+  DAISY_CHECK_LAUNCH();
+  return DAISY_OK;
+}

@@ -109,7 +109,7 @@ void release_workspaces() {
   std::lock_guard<std::mutex> lock(g_mutex);
   g_pool.clear();
 }
-enum { WS_TOKEN = 0, WS_KDA_TOKEN = 1 };
+enum { WS_TOKEN = 0, WS_KDA_TOKEN = 1, WS_PAGED_DECODE = 2 };
 
 // ------------------------------------------------------------------ decode step
 void rope_table(const Tensor& t, const char* name) {
@@ -906,6 +906,147 @@ std::tuple<Tensor, OptTensor, std::vector<Tensor>> kimi_layer(const Tensor& x_, 
   return {y, r.second, out_s};
 }
 
+// ------------------------------------------------------------------ paged cache
+int64_t checked_int(int64_t v, const char* name) {
+  TORCH_CHECK_VALUE(v >= INT32_MIN && v <= INT32_MAX, name, " is out of range");
+  return v;
+}
+const int32_t* ints_of(const Tensor& t, const char* name, int64_t n, const c10::Device& dev) {
+  TORCH_CHECK_VALUE(t.is_cuda() && t.device() == dev, name, " must be a CUDA tensor on ", dev);
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, name, " must be int32, got ", t.scalar_type());
+  TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == n && (n <= 1 || t.stride(0) == 1), name, " must be a contiguous [", n, "] tensor");
+  return t.data_ptr<int32_t>();
+}
+// The pool and its table as the library takes them; page rows are bf16 or float16.
+daisy_b200_pages pages_of(const Tensor& k, const Tensor& v, const Tensor& table, bool* f16) {
+  *f16 = k.scalar_type() == at::kHalf;
+  req(k, "k_pages", *f16 ? at::kHalf : at::kBFloat16); req(v, "v_pages", k.scalar_type());
+  TORCH_CHECK_VALUE(k.dim() == 4 && k.size(3) == 128 && v.sizes() == k.sizes() && v.strides() == k.strides() && v.device() == k.device(),
+                    "k_pages, v_pages must both be [pages, heads, page, 128] with equal strides on one device");
+  TORCH_CHECK_VALUE(k.size(0) >= 1 && k.size(1) >= 1, "a pool has at least one page and one head");
+  const int64_t page = k.size(2);
+  TORCH_CHECK_VALUE(page == 16 || page == 32 || page == 64 || page == 128 || page == 256, "pages hold 16, 32, 64, 128 or 256 rows, got ", page);
+  TORCH_CHECK_VALUE(table.is_cuda() && table.device() == k.device(), "block_table must be a CUDA tensor on ", k.device());
+  TORCH_CHECK_TYPE(table.scalar_type() == at::kInt, "block_table must be int32, got ", table.scalar_type());
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) >= 1 && table.size(1) >= 1 && (table.size(1) == 1 || table.stride(1) == 1) && table.stride(0) >= 0,
+                    "block_table must be [sequences, entries] with contiguous rows");
+  daisy_b200_pages c;
+  c.k = k.data_ptr(); c.v = v.data_ptr();
+  c.p_sb = k.stride(0); c.p_sh = k.stride(1); c.p_sr = k.stride(2);
+  c.table = table.data_ptr<int32_t>(); c.table_sb = table.stride(0);
+  c.n_pages = (int)checked_int(k.size(0), "the pool"); c.H = (int)checked_int(k.size(1), "the pool");
+  c.page = (int)page; c.width = (int)checked_int(table.size(1), "block_table"); c.n_seq = (int)checked_int(table.size(0), "block_table");
+  return c;
+}
+void req_tokens(const Tensor& t, const char* name, int64_t heads, const Tensor& like) {
+  req(t, name);
+  TORCH_CHECK_VALUE(t.device() == like.device(), name, " is on ", t.device(), ", the pages are on ", like.device());
+  TORCH_CHECK_VALUE(t.dim() == 4 && t.size(3) == 128 && (heads < 0 || t.size(2) == heads), name, " must be [B, T, ", heads < 0 ? std::string("H") : std::to_string(heads), ", 128]");
+}
+struct Tables { const float *cos = nullptr, *sin = nullptr; int rows = 0; };
+Tables tables_of(const OptTensor& cos, const OptTensor& sin, int64_t flags, const Tensor& like) {
+  Tables r;
+  if (!(flags & DAISY_ROPE)) return r;
+  TORCH_CHECK_VALUE(cos.has_value() && sin.has_value(), "a rotation needs cos and sin");
+  rope_table(*cos, "cos"); rope_table(*sin, "sin");
+  TORCH_CHECK_VALUE(cos->device() == like.device() && sin->device() == like.device(), "cos, sin must be on ", like.device());
+  r.cos = cos->data_ptr<float>(); r.sin = sin->data_ptr<float>();
+  r.rows = (int)checked_int(std::min(cos->size(0), sin->size(0)), "the RoPE table");
+  return r;
+}
+// value embedding beside v: `ve` viewed as v's shape
+Tensor gate_of(const OptTensor& ve, const OptTensor& gate, const Tensor& v, const float** logit) {
+  *logit = nullptr;
+  if (!ve.has_value()) return Tensor();
+  TORCH_CHECK_VALUE(gate.has_value() && gate->is_cuda() && gate->device() == v.device() && gate->scalar_type() == at::kFloat && gate->numel() == 1,
+                    "ve needs ve_gate_logit, a float32 scalar CUDA tensor");
+  Tensor t = ve->reshape(v.sizes());
+  req(t, "ve");
+  TORCH_CHECK_VALUE(t.device() == v.device(), "ve is on ", t.device(), ", v on ", v.device());
+  *logit = gate->data_ptr<float>();
+  return t;
+}
+// [B, T] of the tokens: one row a sequence, or one packed row
+void req_batch(const Tensor& t, const char* name, bool packed, int64_t n_seq) {
+  TORCH_CHECK_VALUE(!packed || t.size(0) == 1, name, " of packed sequences must be [1, T_total, H, 128]");
+  TORCH_CHECK_VALUE(packed || t.size(0) == n_seq, name, " must have a row for each of the ", n_seq, " sequences of block_table");
+}
+
+OptTensor paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& start, const OptTensor& cos,
+                       const OptTensor& sin, const OptTensor& cu, const OptTensor& q, double eps, int64_t flags, const OptTensor& ve, const OptTensor& ve_gate) {
+  bool f16;
+  const daisy_b200_pages c = pages_of(k_pages, v_pages, table, &f16);
+  c10::cuda::CUDAGuard guard(k_pages.device());
+  req_tokens(k, "k", c.H, k_pages); req_tokens(v, "v", c.H, k_pages);
+  TORCH_CHECK_VALUE(k.size(0) == v.size(0) && k.size(1) == v.size(1), "k and v must be of one shape");
+  req_batch(k, "k", cu.has_value(), c.n_seq);
+  const int64_t B = k.size(0), T = k.size(1);
+  const int32_t* first = ints_of(start, "start", c.n_seq, k_pages.device());
+  const int32_t* cup = cu.has_value() ? ints_of(*cu, "cu_seqlens", c.n_seq + 1, k_pages.device()) : nullptr;
+  TORCH_CHECK_VALUE((flags & ~(int64_t)DAISY_QKV_DEFAULT) == 0, "unknown flags");
+  const Tables rope = tables_of(cos, sin, flags, k_pages);
+  const float* logit;
+  const Tensor vt = gate_of(ve, ve_gate, v, &logit);
+  OptTensor out;
+  int64_t Hq = 0;
+  if (q.has_value()) {
+    req_tokens(*q, "q", -1, k_pages);
+    Hq = q->size(2);
+    TORCH_CHECK_VALUE(q->size(0) == B && q->size(1) == T && Hq >= 1, "q must have the tokens of k");
+    out = at::empty({B, T, Hq, 128}, k_pages.options());
+  }
+  if (T == 0) return out;
+  check(daisy_b200_paged_append(&c, k.data_ptr(), v.data_ptr(), Hq ? q->data_ptr() : nullptr, k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2),
+                                Hq ? q->stride(0) : 0, Hq ? q->stride(1) : 0, Hq ? q->stride(2) : 0, Hq ? out->data_ptr() : nullptr, first, cup, rope.cos, rope.sin, rope.rows,
+                                vt.defined() ? vt.data_ptr() : nullptr, vt.defined() ? vt.stride(0) : 0, vt.defined() ? vt.stride(1) : 0, vt.defined() ? vt.stride(2) : 0, logit,
+                                (int)checked_int(B, "k"), (int)checked_int(T, "k"), (int)Hq, 128, (float)eps, (unsigned)flags | (f16 ? DAISY_CACHE_FP16 : 0), status_ptr(k_pages),
+                                stream_of(k_pages)),
+        "daisy_b200_paged_append");
+  return out;
+}
+
+int64_t paged_decode_workspace_bytes(int64_t n_seq, int64_t Hq, int64_t H) {
+  return (int64_t)daisy_b200_paged_decode_workspace_bytes((int)n_seq, (int)Hq, (int)H, 128);
+}
+
+Tensor paged_decode_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens, int64_t window,
+                         const OptTensor& cos, const OptTensor& sin, double scale, double eps, int64_t flags, const OptTensor& out_, const OptTensor& workspace,
+                         const OptTensor& ve, const OptTensor& ve_gate) {
+  bool f16;
+  const daisy_b200_pages c = pages_of(k_pages, v_pages, table, &f16);
+  c10::cuda::CUDAGuard guard(k_pages.device());
+  req_tokens(q, "q", -1, k_pages); req_tokens(k, "k", c.H, k_pages); req_tokens(v, "v", c.H, k_pages);
+  const int64_t n = c.n_seq, Hq = q.size(2);
+  TORCH_CHECK_VALUE(q.size(0) == n && q.size(1) == 1 && k.size(0) == n && k.size(1) == 1 && v.size(0) == n && v.size(1) == 1, "q, k, v must hold one token for each of the ", n,
+                    " sequences of block_table");
+  TORCH_CHECK_VALUE(Hq >= 1 && Hq % c.H == 0, "query heads (", Hq, ") must be a multiple of the pages' heads (", c.H, ")");
+  const int32_t* len = ints_of(lens, "lens", n, k_pages.device());
+  TORCH_CHECK_VALUE((flags & ~(int64_t)DAISY_QKV_DEFAULT) == 0, "unknown flags");
+  const Tables rope = tables_of(cos, sin, flags, k_pages);
+  const float* logit;
+  const Tensor vt = gate_of(ve, ve_gate, v, &logit);
+  Tensor out;
+  if (out_.has_value()) {
+    out = *out_;
+    req(out, "out");
+    TORCH_CHECK_VALUE(out.device() == k_pages.device() && out.dim() == 4 && out.size(0) == n && out.size(1) == 1 && out.size(2) == Hq && out.size(3) == 128, "out must be [", n,
+                      ", 1, ", Hq, ", 128] on ", k_pages.device());
+  } else {
+    out = at::empty({n, 1, Hq, 128}, q.options());
+  }
+  const int64_t need = paged_decode_workspace_bytes(n, Hq, c.H);
+  if (workspace.has_value())
+    TORCH_CHECK_VALUE(workspace->device() == k_pages.device() && workspace->scalar_type() == at::kByte && workspace->is_contiguous(), "workspace must be contiguous bytes on ",
+                      k_pages.device());
+  Tensor ws = workspace.has_value() ? *workspace : stream_workspace(k_pages, WS_PAGED_DECODE, need);
+  check(daisy_b200_paged_decode_step(&c, q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(2), k.stride(0), k.stride(2), v.stride(0), v.stride(2), len, (int)window,
+                                     rope.cos, rope.sin, rope.rows, out.data_ptr(), out.stride(0), out.stride(2), vt.defined() ? vt.data_ptr() : nullptr,
+                                     vt.defined() ? vt.stride(0) : 0, vt.defined() ? vt.stride(2) : 0, logit, (int)Hq, 128, (float)scale, (float)eps,
+                                     (unsigned)flags | (f16 ? DAISY_CACHE_FP16 : 0), ws.data_ptr(), (size_t)ws.numel(), status_ptr(k_pages), stream_of(k_pages)),
+        "daisy_b200_paged_decode_step");
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -969,6 +1110,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     py::gil_scoped_release released;
     return kimi_layer(x, w, g1_bias, norm_w, conv_w, conv_b, a_log, dt_bias, conv_s, rec, use_cache, silu, eps, H, lengths, mask);
   });
+  m.def("paged_append", &paged_append, nogil());
+  m.def("paged_decode_workspace_bytes", &paged_decode_workspace_bytes);
+  m.def("paged_decode_step", &paged_decode_step, nogil());
   m.def("plain_bf16", &plain_bf16);
   m.def("kda_token_supported", &kda_token_supported);
   m.def("kda_token_workspace_bytes", &kda_token_workspace_bytes);

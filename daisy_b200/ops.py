@@ -414,6 +414,47 @@ def ring_copy_rows(ring_bhcd, lin_bhnd, first_pos: int, to_ring: bool) -> None:
     _lib.check(rc, "daisy_b200_ring_copy_rows")
 
 
+def paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlens: Optional[torch.Tensor] = None,
+                 q: Optional[torch.Tensor] = None, eps: float = 1.1920929e-07, flags: int = QKV_DEFAULT,
+                 ve: Optional[torch.Tensor] = None, ve_gate_logit: Optional[torch.Tensor] = None):
+    """Store the keys and values of new tokens in a paged cache, RMS-normalised and rotated on the way.
+
+    The pool is ``k_pages, v_pages [pages, H, page, 128]`` (bf16 or float16, pages of 16 .. 256 rows, any page / head / row
+    strides); ``block_table [n, entries]`` int32 names the page of positions ``i * page ..`` of each of the ``n`` sequences.
+    ``k, v`` raw ``[n, T, H, 128]`` bf16: ``T`` tokens of every sequence -- or, with ``cu_seqlens`` (int32 ``[n + 1]`` on the
+    device), packed in one row ``[1, T_total, H, 128]``, where tokens past ``cu_seqlens[n]`` belong to nobody.  ``start``
+    int32 ``[n]``: position of each sequence's first new token; a negative one marks an idle sequence, nothing of which is
+    stored.  ``cos, sin`` are whole tables ``[rows, 64]``, indexed by position.
+
+    ``q`` (raw, ``Hq`` heads): returned normalised and rotated, in the pages' type, for :func:`paged_attend`; rows of idle
+    sequences and of nobody's tokens are not written.  ``ve`` with ``ve_gate_logit`` mixes the value embedding into the
+    normalised v as in :func:`qkv_prep`.  Positions outside the block table or the RoPE tables and pages outside the pool are
+    not stored and show up in :func:`check_device_status`.  The index tensors are read on the device only."""
+    return ext().paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlens, q, eps, flags, ve, ve_gate_logit)
+
+
+def paged_decode_workspace(n: int, q_heads: int, heads: int, device) -> torch.Tensor:
+    """Zero-filled workspace of :func:`paged_decode_step` for ``n`` sequences (every call leaves it ready for the next)."""
+    with torch.cuda.device(device):
+        return torch.zeros(ext().paged_decode_workspace_bytes(n, q_heads, heads), dtype=torch.uint8, device=device)
+
+
+def paged_decode_step(q_new, k_new, v_new, k_pages, v_pages, block_table, lens, window: Optional[int], cos, sin,
+                      scale: float = ATTN_SCALE, eps: float = 1.1920929e-07, flags: int = QKV_DEFAULT,
+                      out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                      ve: Optional[torch.Tensor] = None, ve_gate_logit: Optional[torch.Tensor] = None):
+    """One new token of every sequence against a paged cache (see :func:`paged_append`), one launch: ``q_new [n,1,Hq,128]``,
+    ``k_new, v_new [n,1,H,128]`` raw bf16, ``Hq`` a multiple of ``H`` (consecutive query heads share a key head).  ``lens``
+    int32 ``[n]`` on the device: tokens each sequence has in the cache, which is the new one's position; the caller advances it
+    afterwards.  Sees the nearest ``min(lens, window - 1)`` cached rows and its own row, which is stored to its page.  Idle
+    sequences (``lens`` negative) and refused positions give zeros and store nothing.  ``workspace``: from
+    :func:`paged_decode_workspace`, for callers that keep one (a captured graph that is replayed beside other calls);
+    otherwise one is kept per stream.  Nothing depends on host values, so a captured call serves every step.  Returns
+    ``y [n,1,Hq,128]`` bf16."""
+    return ext().paged_decode_step(q_new, k_new, v_new, k_pages, v_pages, block_table, lens, int(window or 0), cos, sin, scale, eps, flags,
+                                   out, workspace, ve, ve_gate_logit)
+
+
 def kda_chunk_fwd(q, k, v, g, beta, scale: Optional[float] = None, initial_state=None,
                   output_final_state: bool = False, l2norm_qk: bool = True, out_fp32: bool = False):
     """KDA chunked forward.  ``q,k [B,T,H,K]`` ``v [B,T,H,V]`` bf16; ``g [B,T,H,K]`` fp32 log-decay; ``beta

@@ -547,6 +547,64 @@ int daisy_b200_kda_token_step(const daisy_b200_kda_layer* layer, const void* x, 
                               void* conv_q, void* conv_k, void* conv_v, int B, int H, int D, float eps, unsigned flags,
                               void* workspace, size_t workspace_bytes, int* status_word, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Paged key-value cache: sequences of uneven length share one pool of pages, for serving batches whose rows stand at
+ * different positions (the reference's KVCache keeps one ring per batch row, all at one position, inference/kv_cache.py:4-68).
+ *   k, v       [n_pages, H, page, D] of bf16, or float16 with DAISY_CACHE_FP16; element strides p_sb (page), p_sh (head),
+ *              p_sr (row), the same for both, D contiguous
+ *   table      int32: position p of sequence b lies in row p % page of page table[b * table_sb + p / page]; entries that no
+ *              visible or new position needs are not read
+ *   page       16, 32, 64, 128 or 256; width entries a sequence
+ * Index arrays (table, start, lens, cu) are read on the device, so a launch can be captured and replayed while they
+ * change.  What they ask for is checked there: a position outside the table's width or the RoPE tables, or a page outside
+ * 0 .. n_pages-1, writes DAISY_EINVAL to the status word; nothing is stored for such a position, a row read from such a
+ * page is taken from page 0. */
+typedef struct daisy_b200_pages {
+  void *k, *v;
+  int64_t p_sb, p_sh, p_sr;
+  const int32_t* table;
+  int64_t table_sb;
+  int n_pages, H, page, width, n_seq;
+} daisy_b200_pages;
+
+/* Keys and values of new tokens to their pages, RMS-normalised and rotated on the way (flags as daisy_b200_qkv_prep); the
+ * tokens' queries, normalised and rotated, to q_out.
+ *   k, v, q    raw projections, logical [B,T,H,D] (q: Hq heads) with strides (s_b,s_t,s_h) each, D contiguous; q and q_out may be NULL
+ *              together
+ *   start      int32 [n_seq]: position of each sequence's first new token, negative: the sequence is idle
+ *   cu         NULL: B = n_seq, sequence b owns the T tokens of row b.  Else B = 1 and int32 [n_seq + 1]: sequence b owns tokens
+ *              cu[b] .. cu[b+1]-1 of the T; tokens at or past cu[n_seq] belong to nobody
+ *   q_out      [B,T,Hq,D] contiguous, in the pages' type; rows of idle sequences and of nobody's tokens are left as they were
+ *   cos, sin   whole tables [table_rows, D/2] float32
+ *   ve, ve_gate_logit   as daisy_b200_qkv_prep, logical [B,T,H,D] beside v; NULL: none */
+int daisy_b200_paged_append(const daisy_b200_pages* cache, const void* k, const void* v, const void* q,
+                            int64_t k_sb, int64_t k_st, int64_t k_sh, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                            int64_t q_sb, int64_t q_st, int64_t q_sh, void* q_out,
+                            const int32_t* start, const int32_t* cu, const float* cos, const float* sin, int table_rows,
+                            const void* ve, int64_t ve_sb, int64_t ve_st, int64_t ve_sh, const float* ve_gate_logit,
+                            int B, int T, int Hq, int D, float eps, unsigned flags, int* status_word, void* stream);
+
+/* One new token of every sequence against its pages: what daisy_b200_swa_decode_step_fused does over a ring.  The token of sequence
+ * b stands at position lens[b]; it sees the nearest min(lens[b], window - 1) cached rows (window <= 0: all) and its own, which is
+ * normalised, rotated, rounded to the pages' type, used at that precision and stored to its page.  One launch.
+ *   q_new      raw, logical [n_seq,1,Hq,D], strides (s_b,s_h); Hq a multiple of the cache's H: query heads g * (Hq/H) ..
+ *              of group g read key head g.  k_new, v_new [n_seq,1,H,D]
+ *   lens       int32 [n_seq]: tokens in the cache, negative: the sequence is idle (its output is zero, nothing is stored); so
+ *              is one whose position is refused
+ *   out        [n_seq,1,Hq,D] bf16 with strides (o_sb,o_sh)
+ *   flags      DAISY_QKV_DEFAULT bits | DAISY_CACHE_FP16
+ *   workspace  daisy_b200_paged_decode_workspace_bytes(n_seq,Hq,H,D) bytes on the current device, 16-byte aligned, zero
+ *              before the first call, afterwards left to the calls.  Calls that may overlap on the device need workspaces of
+ *              their own. */
+size_t daisy_b200_paged_decode_workspace_bytes(int n_seq, int Hq, int H, int D);
+int daisy_b200_paged_decode_step(const daisy_b200_pages* cache, const void* q_new, const void* k_new, const void* v_new,
+                                 int64_t q_sb, int64_t q_sh, int64_t k_sb, int64_t k_sh, int64_t v_sb, int64_t v_sh,
+                                 const int32_t* lens, int window, const float* cos, const float* sin, int table_rows,
+                                 void* out, int64_t o_sb, int64_t o_sh,
+                                 const void* ve, int64_t ve_sb, int64_t ve_sh, const float* ve_gate_logit,
+                                 int Hq, int D, float scale, float eps, unsigned flags,
+                                 void* workspace, size_t workspace_bytes, int* status_word, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
