@@ -40,7 +40,7 @@ constexpr __host__ __device__ int pd_ctas(int cols) { return cols == 8 ? 3 : 2; 
 struct SeqRange { int len, lo, tile0, tiles; };
 __device__ __forceinline__ SeqRange seq_range(const PagedDecodeParams& p, int b) {
   SeqRange r;
-  r.len = p.lens[b];
+  r.len = __ldcg(p.lens + b);                                        // L2: this grid may have been there before they were written
   const bool bad = r.len >= p.c.capacity() || ((p.flags & DAISY_ROPE) && r.len >= p.table_rows);
   if (bad && p.status) p.status[0] = DAISY_EINVAL;
   if (r.len < 0 || bad) r.len = -1;
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
     const int* table = p.c.table + b * p.c.table_sb;
     const int first = r.tile0 + (int)(t - u_at), last = r.tile0 + (int)(s_end - u_at);    // tiles of the sequence
     auto page_of = [&](int tile) -> int {                            // a row outside the pool is taken from page 0
-      int pg = tile < last && r.len > r.lo ? table[(tile * PD_TILE) >> p.c.lg] : 0;
+      int pg = tile < last && r.len > r.lo ? __ldcg(table + ((tile * PD_TILE) >> p.c.lg)) : 0;
       if ((unsigned)pg >= (unsigned)p.c.n_pages) {
         if (p.status) p.status[0] = DAISY_EINVAL;
         pg = 0;
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
         if (warp == 0) {
           *reinterpret_cast<float4*>(&sm_v[4 * lane]) = make_float4(va.x, va.y, vc.x, vc.y);
           if (grp == 0) {
-            const int new_pg = table[r.len >> p.c.lg];
+            const int new_pg = __ldcg(table + (r.len >> p.c.lg));
             if ((unsigned)new_pg < (unsigned)p.c.n_pages) {
               const int64_t at = p.c.at(new_pg, h, r.len) + 8 * lane;
               *reinterpret_cast<uint2*>(p.c.k + at) = k16;

@@ -1,0 +1,870 @@
+// Causal attention of a chunk of every sequence over a paged cache, on tcgen05 tensor cores.
+//
+// Query i of sequence b stands at position lens[b] - n_b + i and sees the nearest `window` keys up to its own, all of them in
+// the pages.  A work item is 256 queries (two 128-row streams that share every K/V tile; 128 where few) of one head; tiles of 128 keys.
+// Long items of a call with few of them are cut along the keys into pieces, whose sums (fp32) the last one to finish joins in
+// a fixed order.  The lengths are on the device, so a first, one-block launch works out the pieces, longest first, and the
+// attention kernel's CTAs draw them one by one.
+//
+// Roles (as in the dense prefill kernel): two softmax warpgroups a stream, 64 key columns each, where the caller bounds the
+// logits (no running maximum is needed then), else one a stream with the whole row and a lazily refreshed reference maximum; a
+// TMA producer; an MMA issuer.  TMEM: S_0 S_1 O_0 O_1, 128 columns each; P overwrites S.
+//
+// K/V tiles come page by page (a box of min(page, 128) rows and 64 channels, 128-byte swizzle); pages that nobody sees are not
+// touched.  What rows of a tile hold that nobody sees (other sequences' old rows, anything) must not reach an output: their
+// scores are replaced, and the issuer clears their V rows in shared memory, since 0 x NaN is NaN in a product.
+// All waits are bounded, as in the dense kernel.
+#include "paged.cuh"
+
+namespace daisy {
+
+constexpr int PP_BM = 128, PP_BN = 128, PP_NSTAGE = 3, PP_NQBUF = 2, PP_NITEM = 3;
+constexpr int PP_TILE = PP_BM * DAISY_HEAD_DIM * 2, PP_HALF = PP_TILE / 2;      // 32 KB; one [128 x 64] swizzled box
+constexpr int PP_SMEM_TILES = (2 * PP_NQBUF + PP_NSTAGE) * PP_TILE;
+constexpr int PP_BARS = 640;
+constexpr int PP_SMEM = 1024 + PP_SMEM_TILES + PP_BARS;
+static_assert(PP_SMEM <= 232448, "over the 227 KB a CTA may use");
+constexpr float PP_NEG = -1.0e30f;
+
+// A piece: key tiles j0 .. j1 of the 256 (or 128) queries i0 .. of sequence b.  parts > 1: one of several, at slot + head * parts + part.
+struct __align__(32) Piece { int b, i0, j0, j1, slot, part, parts, pad; };
+
+struct PlanHead { int n_pieces, queue, pad[6]; };
+
+struct PagedPrefillParams {
+  PagedCache c;
+  __nv_bfloat16* out;
+  int64_t o_sb, o_st, o_sh;
+  const int *lens, *cu;
+  int T, Hq, G, window, rows;        // rows: queries of an item
+  float scale_log2;
+  int* status;
+  PlanHead* head;
+  Piece* pieces;
+  float* part;                       // [slots][PP_SLOT]
+  int* tickets;                      // [slots][16], zero between calls
+  int slots, max_pieces;
+};
+// a warp's share of a piece's sums: [columns][32 rows], then reference and denominator of the 32 rows
+constexpr int PP_SLOT = 2 * 8 * (64 * 32 + 64);                     // floats: 8 warps a stream x 64 columns (or 4 x 128)
+
+// Queries and keys of sequence b: n queries at positions pos .. , n = 0 where there are none; pos < 0: nothing to see (idle, or refused).
+struct SeqQueries { int n, row0, pos; bool refused; };
+__device__ __forceinline__ SeqQueries seq_queries(const PagedPrefillParams& p, int b) {
+  SeqQueries s;
+  if (p.cu) {
+    const int a = __ldcg(p.cu + b), e = __ldcg(p.cu + b + 1);
+    const bool sane = a >= 0 && e >= a && e <= p.T;                  // offsets outside the row: the sequence has no queries
+    s.n = sane ? e - a : 0;
+    s.row0 = sane ? a : 0;
+    s.refused = !sane;
+  } else {
+    s.n = p.T; s.row0 = 0; s.refused = false;
+  }
+  const int len = __ldcg(p.lens + b);
+  s.pos = len - s.n;
+  if (len < 0) s.pos = -1;
+  else if (len < s.n || len > p.c.capacity()) { s.pos = -1; s.refused = s.refused || s.n > 0; }
+  return s;
+}
+// key tiles that queries at positions pos .. pos + n - 1 see
+__device__ __forceinline__ int first_tile(int pos, int window) { return (window > 0 ? max(0, pos - window + 1) : 0) / PP_BN; }
+__device__ __forceinline__ int last_tile(int pos, int n) { return (pos + n - 1) / PP_BN; }
+
+// The pieces of a call, longest first.  One block; a warp a sequence, a lane an item.
+// How far items are cut: into pieces of at most L tiles, L from a few candidates by the estimate
+// total / CTAs + half a longest piece (+ four tiles' time for every piece of a cut item), or a longest piece where all pieces find a CTA.
+constexpr int PLAN_THREADS = 1024, PLAN_CAND = 6, PLAN_BUCKETS = 1024;
+__global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PagedPrefillParams p, int ctas) {
+  __shared__ int hist[PLAN_BUCKETS];
+  __shared__ unsigned long long sm_total;
+  __shared__ int sm_longest, sm_items, sm_slots, sm_cut, sm_pieces[PLAN_CAND], sm_parts[PLAN_CAND], sm_L[PLAN_CAND];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < PLAN_BUCKETS; i += PLAN_THREADS) hist[i] = 0;
+  if (threadIdx.x == 0) { sm_total = 0; sm_longest = 0; sm_items = 0; sm_slots = 0; }
+  if (threadIdx.x < PLAN_CAND) { sm_pieces[threadIdx.x] = 0; sm_parts[threadIdx.x] = 0; }
+  grid_dep_launch();
+  grid_dep_wait();
+  __syncthreads();
+  // f(b, i0, j0, j1) for every item; j1 < j0: rows that see nothing
+  auto items = [&](auto f) {
+    for (int b = warp; b < p.c.n_seq; b += PLAN_THREADS / 32) {
+      const SeqQueries s = seq_queries(p, b);
+      if (s.refused && p.status && lane == 0) p.status[0] = DAISY_EINVAL;
+      for (int i0 = lane * p.rows; i0 < s.n; i0 += 32 * p.rows) {
+        if (s.pos < 0) f(b, i0, 1, 0);
+        else f(b, i0, first_tile(s.pos + i0, p.window), last_tile(s.pos + i0, min(p.rows, s.n - i0)));
+      }
+    }
+  };
+  {
+    unsigned long long total = 0;
+    int longest = 0, n = 0;
+    items([&](int, int, int j0, int j1) { const int t = j1 - j0 + 1; total += t; longest = max(longest, t); ++n; });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+      longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+      n += __shfl_xor_sync(0xffffffffu, n, o);
+    }
+    if (lane == 0 && n > 0) { atomicAdd(&sm_total, total); atomicMax(&sm_longest, longest); atomicAdd(&sm_items, n); }
+  }
+  __syncthreads();
+  if (threadIdx.x < PLAN_CAND) {
+    const int fit = sm_items > 0 ? ctas / max(1, sm_items * p.Hq) : 1;
+    const int n = threadIdx.x == 0 ? 1 : threadIdx.x == 1 ? max(1, fit) : threadIdx.x;             // whole; as many as find a CTA; 2, 3, 4, 5
+    sm_L[threadIdx.x] = max((sm_longest + n - 1) / n, min(4, max(sm_longest, 1)));
+  }
+  __syncthreads();
+  {
+    int pieces[PLAN_CAND] = {}, parts[PLAN_CAND] = {};
+    items([&](int, int, int j0, int j1) {
+      const int t = max(j1 - j0 + 1, 1);
+#pragma unroll
+      for (int k = 0; k < PLAN_CAND; ++k) {
+        const int n = (t + sm_L[k] - 1) / sm_L[k];
+        pieces[k] += n;
+        if (n > 1) parts[k] += n;
+      }
+    });
+#pragma unroll
+    for (int k = 0; k < PLAN_CAND; ++k) {
+      if (pieces[k]) atomicAdd(&sm_pieces[k], pieces[k]);
+      if (parts[k]) atomicAdd(&sm_parts[k], parts[k]);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float best = 3.0e38f;
+    int cut = 0;
+    for (int k = 0; k < PLAN_CAND; ++k) {
+      const int64_t n = (int64_t)sm_pieces[k] * p.Hq, parts = (int64_t)sm_parts[k] * p.Hq;
+      if (k > 0 && (parts > p.slots || sm_pieces[k] > p.max_pieces)) continue;
+      const float share = (float)sm_total * p.Hq / ctas;
+      const float est = (n <= ctas ? (float)sm_L[k] : share + 0.5f * sm_L[k]) + (parts > 0 ? 4.f * fmaxf(1.f, (float)parts / ctas) : 0.f);
+      if (est < best) { best = est; cut = sm_L[k]; }
+    }
+    sm_cut = cut;
+  }
+  __syncthreads();
+  const int L = max(sm_cut, 1);
+  auto bucket = [](int t) { return PLAN_BUCKETS - 1 - min(max(t, 0), PLAN_BUCKETS - 1); };          // longest first
+  auto pieces_of = [&](int j0, int j1, auto f) {
+    const int t = j1 - j0 + 1, n = max(1, (t + L - 1) / L);
+    for (int i = 0; i < n; ++i) f(j0 + (int)((int64_t)t * i / n), n == 1 ? j1 : j0 + (int)((int64_t)t * (i + 1) / n) - 1, i, n);
+  };
+  items([&](int, int, int j0, int j1) { pieces_of(j0, j1, [&](int a, int e, int, int) { atomicAdd(&hist[bucket(e - a + 1)], 1); }); });
+  __syncthreads();
+  // exclusive prefix sums of the 1024 buckets
+  __shared__ int warp_sums[32];
+  {
+    const int own = hist[threadIdx.x];
+    int x = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    int base = 0;
+    for (int w = 0; w < warp; ++w) base += warp_sums[w];
+    hist[threadIdx.x] = base + x - own;
+    if (threadIdx.x == PLAN_THREADS - 1) { p.head->n_pieces = min(base + x, p.max_pieces); p.head->queue = 0; }
+  }
+  __syncthreads();
+  items([&](int b, int i0, int j0, int j1) {
+    const int n = max(1, (j1 - j0 + L) / L);
+    const int slot = n > 1 ? atomicAdd(&sm_slots, n * p.Hq) : 0;
+    pieces_of(j0, j1, [&](int a, int e, int i, int parts) {
+      const int at = atomicAdd(&hist[bucket(e - a + 1)], 1);
+      if (at < p.max_pieces) p.pieces[at] = Piece{b, i0, a, e, slot, i, parts, 0};
+    });
+  });
+}
+
+struct PagedItem {
+  int b, h;                          // b < 0: no more
+  int q0[2], n[2], jlo_s[2], jhi_s[2];
+  bool valid[2];                     // has tiles in this piece
+  int jlo, jhi;
+  int see0, end;                     // keys see0 .. end - 1 are seen by some row of the item
+  int row0, bq;                      // first row of stream 0: token and batch row of q and out
+  int slot, parts, part;
+};
+
+struct PagedBarriers {
+  uint64_t q_full[2][PP_NQBUF], q_empty[2][PP_NQBUF];
+  uint64_t kv_full[PP_NSTAGE], kv_empty[PP_NSTAGE];
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t l_full[2][4];             // the partial row sums of the two warps that share 32 rows of a stream
+  uint64_t i_full[PP_NITEM], i_empty[PP_NITEM];
+  PagedItem item[PP_NITEM];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(PagedBarriers) <= PP_BARS, "room for the barriers");
+
+// NSPLIT = 2: bounded logits, two warps (64 columns each) for 32 rows; NSPLIT = 1: any logits, one warp.
+template <int NSPLIT, bool F16>
+__global__ void __launch_bounds__(32 * (8 * NSPLIT + 2), 1)
+paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v, const PagedPrefillParams p) {
+  static_assert(!(F16 && NSPLIT == 2), "weights without a reference maximum do not fit float16");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_tiles = smem;
+  uint8_t* kv_tiles = smem + 2 * PP_NQBUF * PP_TILE;
+  PagedBarriers* bars = reinterpret_cast<PagedBarriers*>(smem + PP_SMEM_TILES);
+  volatile int* abort_flag = &bars->abort_flag;
+  constexpr int TMA_WARP = 8 * NSPLIT, MMA_WARP = 8 * NSPLIT + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      for (int qb = 0; qb < PP_NQBUF; ++qb) { mbar_init(&bars->q_full[s][qb], 1); mbar_init(&bars->q_empty[s][qb], 4 * NSPLIT); }
+      mbar_init(&bars->s_full[s], 1);
+      mbar_init(&bars->p_full[s], 128 * NSPLIT);
+      mbar_init(&bars->o_full[s], 1);
+      for (int i = 0; i < 4; ++i) mbar_init(&bars->l_full[s][i], 2);
+    }
+    for (int i = 0; i < PP_NSTAGE; ++i) { mbar_init(&bars->kv_full[i], 1); mbar_init(&bars->kv_empty[i], 1); }
+    for (int i = 0; i < PP_NITEM; ++i) { mbar_init(&bars->i_full[i], 1); mbar_init(&bars->i_empty[i], 8 * NSPLIT + 1); }
+    bars->abort_flag = 0;
+    mbar_init_fence();
+  }
+  if (warp == MMA_WARP) {
+    tmem_alloc(&bars->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+  grid_dep_launch();
+  grid_dep_wait();
+
+  auto next_item = [&](int rd) -> const PagedItem* {
+    const PagedItem* g = &bars->item[rd % PP_NITEM];
+    if (!__all_sync(0xffffffffu, mbar_wait(&bars->i_full[rd % PP_NITEM], (rd / PP_NITEM) & 1, abort_flag, p.status, 13))) return nullptr;
+    return g->b >= 0 ? g : nullptr;
+  };
+  auto item_done = [&](int rd) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->i_empty[rd % PP_NITEM]);
+  };
+
+  if (warp == TMA_WARP) {
+    // ------------------------------------------------------------------ TMA producer: the warp as one, lane 0 issues
+    if (lane == 0) { prefetch_tmap(&tm_q); prefetch_tmap(&tm_k); prefetch_tmap(&tm_v); }
+    const int n_work = __ldcg(&p.head->n_pieces) * p.Hq;            // L2: this grid was there before the plan was written
+    int n = 0;
+    uint32_t qn[2] = {0, 0};
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, where)) != 0;
+    };
+    auto load_q = [&](const PagedItem& g) {
+      for (int s = 0; s < 2 && ok; ++s) {
+        if (!g.valid[s]) continue;
+        const int qb = qn[s] % PP_NQBUF;
+        if (!wait(&bars->q_empty[s][qb], ((qn[s] / PP_NQBUF) & 1) ^ 1, 9)) { ok = false; break; }
+        ++qn[s];
+        uint8_t* dst = q_tiles + (qb * 2 + s) * PP_TILE;
+        if (lane == 0) {
+          mbar_expect_tx(&bars->q_full[s][qb], PP_TILE);
+          tma_load_4d(dst, &tm_q, &bars->q_full[s][qb], 0, g.row0 + s * PP_BM, g.h, g.bq);
+          tma_load_4d(dst + PP_HALF, &tm_q, &bars->q_full[s][qb], 64, g.row0 + s * PP_BM, g.h, g.bq);
+        }
+      }
+    };
+    int drawn = blockIdx.x;                                         // the first one is this CTA's own number, later ones are drawn
+    auto draw = [&]() {
+      int x = 0;
+      if (lane == 0) x = atomicAdd(&p.head->queue, 1);
+      drawn = (int)gridDim.x + __shfl_sync(0xffffffffu, x, 0);
+    };
+    auto publish = [&](int rd, PagedItem& g) {
+      const int slot = rd % PP_NITEM;
+      g.b = -1;
+      if (drawn < n_work) {
+        const int at = drawn / p.Hq;
+        const int4* src = reinterpret_cast<const int4*>(p.pieces + at);
+        const int4 lo = __ldcg(src), hi = __ldcg(src + 1);
+        const Piece pc{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        const SeqQueries sq = seq_queries(p, pc.b);
+        g.b = pc.b; g.h = drawn - at * p.Hq;
+        g.bq = p.cu ? 0 : pc.b;
+        g.row0 = sq.row0 + pc.i0;
+        g.slot = pc.slot + g.h * pc.parts; g.part = pc.part; g.parts = pc.parts;
+        const int pos = sq.pos + pc.i0;
+        g.jlo = 1 << 30; g.jhi = -1;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          g.q0[s] = pos + s * PP_BM;
+          g.n[s] = min(max(min(p.rows, sq.n - pc.i0) - s * PP_BM, 0), PP_BM);
+          g.jlo_s[s] = 1; g.jhi_s[s] = 0;
+          if (g.n[s] > 0 && sq.pos >= 0) {
+            g.jlo_s[s] = max(first_tile(g.q0[s], p.window), pc.j0);
+            g.jhi_s[s] = min(last_tile(g.q0[s], g.n[s]), pc.j1);
+          }
+          g.valid[s] = g.jhi_s[s] >= g.jlo_s[s];
+          if (g.valid[s]) { g.jlo = min(g.jlo, g.jlo_s[s]); g.jhi = max(g.jhi, g.jhi_s[s]); }
+        }
+        g.see0 = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+        g.end = pos + g.n[0] + g.n[1];
+      }
+      if (!wait(&bars->i_empty[slot], ((rd / PP_NITEM) & 1) ^ 1, 14)) { ok = false; return; }
+      if (lane == 0) {
+        bars->item[slot] = g;
+        mbar_arrive(&bars->i_full[slot]);
+      }
+      if (g.b >= 0) draw();
+    };
+    PagedItem g, g_next;
+    publish(0, g);
+    if (ok && g.b >= 0) load_q(g);
+    for (int rd = 0; ok && g.b >= 0; ++rd, g = g_next) {
+      // the table's entries, 32 at a time, the next 32 on their way
+      const int* table = p.c.table + g.b * p.c.table_sb;
+      const int e_first = g.see0 >> p.c.lg, e_last = (g.end - 1) >> p.c.lg;
+      auto entries = [&](int from) {
+        const int i = from + lane;
+        return i >= e_first && i <= e_last ? __ldcg(table + i) : 0;
+      };
+      int from = max((g.jlo * PP_BN) >> p.c.lg, 0);
+      int cur = 0, ahead = 0;
+      if (g.jhi >= g.jlo) { cur = entries(from); ahead = entries(from + 32); }
+      auto page_of = [&](int e) {                                    // e not below `from`
+        while (e >= from + 32) { from += 32; cur = ahead; ahead = entries(from + 32); }
+        int pg = __shfl_sync(0xffffffffu, cur, e - from);
+        if ((unsigned)pg >= (unsigned)p.c.n_pages) {
+          if (p.status && lane == 0) p.status[0] = DAISY_EINVAL;
+          pg = 0;
+        }
+        return pg;
+      };
+      bool next_out = false;
+      for (int j = g.jlo; j <= g.jhi && ok; ++j) {
+        const int rows = min(1 << p.c.lg, PP_BN), boxes = PP_BN / rows;
+        const int k0 = j * PP_BN;
+        // boxes that hold a row somebody sees
+        const int b_first = max(g.see0 - k0, 0) / rows, b_last = (min(g.end - k0, PP_BN) - 1) / rows;
+        int pages[8];
+        const int e_lo = k0 >> p.c.lg;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          pages[i] = 0;
+          if (i < boxes && i >= b_first && i <= b_last) pages[i] = page_of(e_lo + (rows < PP_BN ? i : 0));
+        }
+        const uint32_t bytes = (uint32_t)(b_last - b_first + 1) * rows * 256u;
+        for (int kv = 0; kv < 2; ++kv, ++n) {
+          const int stage = n % PP_NSTAGE;
+          if (!wait(&bars->kv_empty[stage], ((n / PP_NSTAGE) & 1) ^ 1, 1)) { ok = false; break; }
+          if (lane == 0) {
+            uint8_t* dst = kv_tiles + stage * PP_TILE;
+            const CUtensorMap* tm = kv ? &tm_v : &tm_k;
+            mbar_expect_tx(&bars->kv_full[stage], bytes);
+            const int in_page = k0 & ((1 << p.c.lg) - 1);            // of a page longer than a tile
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (i >= b_first && i <= b_last) {
+                tma_load_4d(dst + i * rows * 128, tm, &bars->kv_full[stage], 0, in_page, g.h / p.G, pages[i]);
+                tma_load_4d(dst + PP_HALF + i * rows * 128, tm, &bars->kv_full[stage], 64, in_page, g.h / p.G, pages[i]);
+              }
+          }
+          __syncwarp();
+        }
+        if (ok && j == g.jhi) {                                      // the next item's queries, when this one's last tiles are asked for
+          publish(rd + 1, g_next);
+          if (ok && g_next.b >= 0) load_q(g_next);
+          next_out = true;
+        }
+      }
+      if (ok && !next_out) {                                         // an item without tiles
+        publish(rd + 1, g_next);
+        if (ok && g_next.b >= 0) load_q(g_next);
+      }
+    }
+  } else if (warp == MMA_WARP) {
+    // ------------------------------------------------------------------ MMA issuer.  Per tile: PV_0(j-1) QK_0(j) PV_1(j-1) QK_1(j)
+    const uint32_t leader = elect_one() ? 1u : 0u;
+    constexpr uint32_t idesc_qk = F16 ? umma_idesc_f16(PP_BM, PP_BN, 0, 0) : umma_idesc_bf16(PP_BM, PP_BN, 0, 0);
+    constexpr uint32_t idesc_pv = F16 ? umma_idesc_f16(PP_BM, DAISY_HEAD_DIM, 0, 1) : umma_idesc_bf16(PP_BM, DAISY_HEAD_DIM, 0, 1);
+    const uint64_t qd = umma_desc_sw128(smem_u32(q_tiles), 16, 1024);
+    const uint64_t kd = umma_desc_sw128(smem_u32(kv_tiles), 16, 1024);
+    const uint64_t vd = umma_desc_sw128(smem_u32(kv_tiles), PP_HALF, 1024);
+    const uint32_t q_lo0 = (uint32_t)qd, k_lo0 = (uint32_t)kd, qk_hi = (uint32_t)(qd >> 32);
+    const uint32_t v_lo0 = (uint32_t)vd, v_hi = (uint32_t)(vd >> 32);
+    int n_base = 0;
+    uint32_t n_pv[2] = {0, 0}, n_q[2] = {0, 0};
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, where)) != 0;
+    };
+    const PagedItem* item;
+    for (int rd = 0; ok && (item = next_item(rd)); ++rd) {
+      const PagedItem g = *item;
+      item_done(rd);
+      if (g.jhi < g.jlo) continue;
+      for (int j = g.jlo; j <= g.jhi + 1 && ok; ++j) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (!g.valid[s]) continue;
+          const uint32_t s_tmem = tmem_base + s * 128, o_tmem = tmem_base + 256 + s * 128;
+          if (j - 1 >= g.jlo_s[s] && j - 1 <= g.jhi_s[s]) {          // O_s += P_s(j-1) V_{j-1}
+            const int n = n_base + 2 * (j - 1 - g.jlo) + 1, stage = n % PP_NSTAGE;
+            if (!wait(&bars->p_full[s], n_pv[s] & 1, 2)) { ok = false; break; }
+            ++n_pv[s];
+            const bool v_seen = s == 1 && g.valid[0] && j - 1 >= g.jlo_s[0] && j - 1 <= g.jhi_s[0];
+            if (!v_seen) {
+              if (!wait(&bars->kv_full[stage], (n / PP_NSTAGE) & 1, 3)) { ok = false; break; }
+              const int k0 = (j - 1) * PP_BN, lo = max(g.see0 - k0, 0), hi = min(g.end - k0, PP_BN);
+              if (lo > 0 || hi < PP_BN) {                            // rows that nobody sees
+                uint8_t* tile = kv_tiles + stage * PP_TILE + (lane & 7) * 16;
+                for (int r = lane >> 3; r < PP_BN; r += 4)
+                  if (r < lo || r >= hi) {
+                    *reinterpret_cast<uint4*>(tile + r * 128) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(tile + PP_HALF + r * 128) = make_uint4(0, 0, 0, 0);
+                  }
+                fence_proxy_async();
+                __syncwarp();
+              }
+            }
+            tc_fence_after();
+            const uint32_t v_lo = v_lo0 + stage * (PP_TILE >> 4);
+            umma_ts_lh_p(leader, o_tmem, s_tmem, v_lo, v_hi, idesc_pv, j - 1 == g.jlo_s[s] ? 0u : 1u);
+#pragma unroll
+            for (int k = 1; k < PP_BN / 16; ++k)
+              umma_ts_lh_p(leader, o_tmem, s_tmem + (NSPLIT == 2 ? (k & 3) * 8 + (k >> 2) * 64 : k * 8), v_lo + k * (2048 >> 4), v_hi, idesc_pv, 1u);
+            const bool other_uses = s == 0 && g.valid[1] && j - 1 >= g.jlo_s[1] && j - 1 <= g.jhi_s[1];
+            if (!other_uses) tc_commit_p(leader, &bars->kv_empty[stage]);
+            if (j - 1 == g.jhi_s[s]) tc_commit_p(leader, &bars->o_full[s]);
+          }
+          if (j >= g.jlo_s[s] && j <= g.jhi_s[s]) {                  // S_s = Q_s K_j^T
+            const int n = n_base + 2 * (j - g.jlo), stage = n % PP_NSTAGE;
+            if (j == g.jlo_s[s]) {
+              const uint32_t qb = n_q[s] % PP_NQBUF;
+              if (!wait(&bars->q_full[s][qb], (n_q[s] / PP_NQBUF) & 1, 4)) { ok = false; break; }
+              ++n_q[s];
+            }
+            const bool k_seen = s == 1 && g.valid[0] && j >= g.jlo_s[0] && j <= g.jhi_s[0];
+            if (!k_seen && !wait(&bars->kv_full[stage], (n / PP_NSTAGE) & 1, 5)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t q_buf = (n_q[s] - 1) % PP_NQBUF;
+            const uint32_t q_lo = q_lo0 + (q_buf * 2 + s) * (PP_TILE >> 4), k_lo = k_lo0 + stage * (PP_TILE >> 4);
+#pragma unroll
+            for (int k = 0; k < DAISY_HEAD_DIM / 16; ++k) {
+              const uint32_t off = ((k >> 2) * PP_HALF + (k & 3) * 32) >> 4;
+              umma_ss_lh_p(leader, s_tmem, q_lo + off, qk_hi, k_lo + off, qk_hi, idesc_qk, k > 0 ? 1u : 0u);
+            }
+            tc_commit_p(leader, &bars->s_full[s]);
+            const bool other_uses = s == 0 && g.valid[1] && j >= g.jlo_s[1] && j <= g.jhi_s[1];
+            if (!other_uses) tc_commit_p(leader, &bars->kv_empty[stage]);
+          }
+        }
+      }
+      n_base += 2 * (g.jhi - g.jlo + 1);
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax + epilogue
+    constexpr int COLS = 128 / NSPLIT;                               // of the scores, and of the output in the epilogue
+    const int grp = warp >> 2, quarter = warp & 3;
+    const int s = NSPLIT == 2 ? grp & 1 : grp, half = NSPLIT == 2 ? grp >> 1 : 0;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_tmem = tmem_base + lane_off + s * 128 + half * 64;
+    const uint32_t o_tmem = tmem_base + lane_off + 256 + s * 128 + half * 64;
+    const float c2 = p.scale_log2;
+    uint32_t n_s = 0, n_o = 0;
+    bool ok = true;
+    const PagedItem* item;
+
+    // rows of this warp to the output, straight from registers
+    auto store_row = [&](const PagedItem* g, const float* y) {       // y: COLS values of this lane's row
+      if (row >= g->n[s]) return;
+      __nv_bfloat16* dst = p.out + g->bq * p.o_sb + (int64_t)(g->row0 + s * PP_BM + row) * p.o_st + g->h * p.o_sh + half * 64;
+#pragma unroll
+      for (int c = 0; c < COLS; c += 8) *reinterpret_cast<uint4*>(dst + c) = pack8(y + c);
+    };
+    // this warp's share of a cut item: left in the slot; the last warp to come joins the pieces in their order
+    auto join = [&](const PagedItem* g, const uint32_t* o, float m, float l) {
+      constexpr int SHARE = COLS * 32 + 64;
+      auto share = [&](int part) { return p.part + (int64_t)(g->slot + part) * PP_SLOT + ((s * NSPLIT + half) * 4 + quarter) * SHARE; };
+      float* dst = share(g->part);
+      if (l > 0.f || !(l == l)) {
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) dst[c * 32 + lane] = __uint_as_float(o[c]);
+      }
+      dst[COLS * 32 + lane] = m;
+      dst[COLS * 32 + 32 + lane] = l;
+      __threadfence();
+      __syncwarp();
+      int last = 0;
+      if (lane == 0) {
+        int* tk = p.tickets + (int64_t)g->slot * 16 + (s * NSPLIT + half) * 4 + quarter;
+        last = atomicAdd(tk, 1) == g->parts - 1;
+        if (last) *tk = 0;
+      }
+      if (!__shfl_sync(0xffffffffu, last, 0)) return;
+      __threadfence();
+      float y[COLS], M = PP_NEG, den = 0.f;
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) y[c] = 0.f;
+      for (int i = 0; i < g->parts; ++i) {
+        const float* src = share(i);
+        const float m1 = __ldcg(src + COLS * 32 + lane), l1 = __ldcg(src + COLS * 32 + 32 + lane);
+        if (l1 == 0.f) continue;                                     // this lane's row sees none of that piece
+        const float top = fmaxf(M, m1), a = fast_exp2(M - top), e = fast_exp2(m1 - top);
+        den = den * a + l1 * e;
+        M = top;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) y[c] = y[c] * a + __ldcg(src + c * 32 + lane) * e;
+      }
+      const float inv = 1.0f / den;
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) y[c] *= inv;
+      store_row(g, y);
+    };
+    // rows of an item that this warp's stream has no tiles of
+    auto without_tiles = [&](const PagedItem* g) {
+      if (g->n[s] == 0) return;
+      uint32_t zero[COLS];
+      float none[COLS];
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) { zero[c] = 0; none[c] = 0.f; }
+      if (g->parts > 1) join(g, zero, PP_NEG, 0.f);
+      else store_row(g, none);
+    };
+    // the last step of an item: l, m of this lane's row, sums in O.  box: 32 rows of 128 bytes (two with NSPLIT = 1) of the item's Q buffer,
+    // which its last scores have left, turn the lanes' rows into whole row segments
+    auto finish = [&](const PagedItem* g, float m, float l, uint8_t* box) {
+      uint32_t o[COLS];
+#pragma unroll
+      for (int c = 0; c < COLS; c += 32) tmem_ld32(o_tmem + c, o + c);
+      tc_wait_ld();
+      if (g->parts > 1) {
+        join(g, o, m, l);
+      } else {
+        const float inv = 1.0f / l;
+        __nv_bfloat16* dst = p.out + g->bq * p.o_sb + (int64_t)(g->row0 + s * PP_BM + quarter * 32) * p.o_st + g->h * p.o_sh + half * 64 + (lane & 7) * 8;
+        const int n_rows = g->n[s] - quarter * 32;
+#pragma unroll
+        for (int hc = 0; hc < COLS / 64; ++hc) {
+          uint8_t* mine = box + hc * PP_HALF;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(o[hc * 64 + 8 * c + e]) * inv;
+            *reinterpret_cast<uint4*>(mine + row * 128 + ((c ^ (row & 7)) << 4)) = pack8(y);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            const uint4 v = *reinterpret_cast<const uint4*>(mine + (quarter * 32 + r) * 128 + (((lane & 7) ^ (r & 7)) << 4));
+            if (r < n_rows) *reinterpret_cast<uint4*>(dst + (int64_t)r * p.o_st + hc * 64) = v;
+          }
+        }
+      }
+      // the next item's first product into O_s follows this warp's next weights, which follow these loads
+      tc_fence_before();
+      fence_proxy_async();                                           // the Q buffer is next written by a copy
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->q_empty[s][n_o % PP_NQBUF]);
+      ++n_o;
+    };
+
+    for (int rd = 0; ok && (item = next_item(rd)); item_done(rd), ++rd) {
+      const int q0 = item->q0[s], jlo = item->jlo_s[s], jhi = item->jhi_s[s];
+      if (jhi < jlo) { without_tiles(item); continue; }
+      const int q_row = q0 + row;
+      uint8_t* q_buf = q_tiles + ((n_o % PP_NQBUF) * 2 + s) * PP_TILE;
+      auto scores_there = [&]() -> bool {
+        const bool there = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[s], n_s & 1, abort_flag, p.status, 6));
+        ++n_s;
+        tc_fence_after();
+        return there;
+      };
+      auto weights_done = [&]() {
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bars->p_full[s]);
+      };
+      // whole tiles: all rows of the stream see all of their keys
+      const int f_lo = p.window > 0 ? max(q0 + PP_BM + PP_BN - 1 - p.window, 0) / PP_BN : 0, f_hi = (q0 + 1) / PP_BN - 1;
+      if constexpr (NSPLIT == 2) {
+        const uint64_t c2p = pack2f(c2, c2);
+        uint64_t sum_a = pack2f(0.f, 0.f), sum_b = sum_a;
+        auto rebuild = [&](uint32_t (&r)[64], int c) {               // weights of 32 columns and their share of the row sums
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            if (c == 0 && i == 16) tmem_ld32(s_tmem + 32, r + 32);   // the other half of the scores, under this one
+            const uint64_t xa = fmul2(pack2f(__uint_as_float(r[32 * c + i]), __uint_as_float(r[32 * c + i + 1])), c2p);
+            const uint64_t xb = fmul2(pack2f(__uint_as_float(r[32 * c + i + 2]), __uint_as_float(r[32 * c + i + 3])), c2p);
+            float x0, x1, p2, p3;
+            unpack2f(xa, x0, x1);
+            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+            uint64_t pb;
+            if (i & 4) {                                             // one pair in four goes to the FMA pipes
+              pb = exp2_poly2(xb);
+              unpack2f(pb, p2, p3);
+            } else {
+              float x2, x3;
+              unpack2f(xb, x2, x3);
+              p2 = fast_exp2(x2); p3 = fast_exp2(x3);
+              pb = pack2f(p2, p3);
+            }
+            sum_a = fadd2(sum_a, pack2f(p0, p1));
+            sum_b = fadd2(sum_b, pb);
+            pk[i >> 1] = pack_bf16(p0, p1);
+            pk[(i >> 1) + 1] = pack_bf16(p2, p3);
+          }
+          tmem_st16(s_tmem + 16 * c, pk);
+          if (c == 0) tc_wait_ld();
+        };
+        for (int j = jlo; ok && j <= jhi;) {
+          if (j >= f_lo && j <= f_hi) {
+            int run = min(f_hi, jhi) + 1 - j;
+            j += run;
+            for (; run > 0; --run) {
+              ok = scores_there();
+              if (!ok) break;
+              uint32_t r[64];
+              tmem_ld32(s_tmem, r);
+              tc_wait_ld();
+              rebuild(r, 0);
+              rebuild(r, 1);
+              weights_done();
+            }
+            if (!ok) break;
+          } else {
+            ok = scores_there();
+            if (!ok) break;
+            uint32_t r[64];
+            tmem_ld32(s_tmem, r);
+            tc_wait_ld();
+            const int hi = q_row - (j * PP_BN + half * 64), lo = p.window > 0 ? hi - p.window : -1;      // column i is visible iff lo < i <= hi
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              if (!__any_sync(0xffffffffu, hi >= 32 * c && lo < 32 * c + 31)) {
+                const uint32_t zero[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+                if (c == 0) tmem_ld32(s_tmem + 32, r + 32);
+                tmem_st16(s_tmem + 16 * c, zero);
+                if (c == 0) tc_wait_ld();
+                continue;
+              }
+              if (!__all_sync(0xffffffffu, hi >= 32 * c + 31 && lo < 32 * c)) {
+                const int b_lo = min(max(lo + 1 - 32 * c, 0), 32), b_hi = min(max(hi + 1 - 32 * c, 0), 32);
+                const uint32_t visible = (uint32_t)(((uint64_t)1 << b_hi) - 1) & ~(uint32_t)(((uint64_t)1 << b_lo) - 1);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (!((visible >> i) & 1u)) r[32 * c + i] = 0xff800000u;      // -inf -> weight 0
+              }
+              rebuild(r, c);
+            }
+            weights_done();
+            ++j;
+          }
+        }
+        if (!ok) break;
+        float a0, a1, b0, b1;
+        unpack2f(sum_a, a0, a1);
+        unpack2f(sum_b, b0, b1);
+        float l = (a0 + a1) + (b0 + b1);
+        // the two warps that share rows exchange their sums through the item's Q buffer, each into the rows that the other's output will take
+        *reinterpret_cast<float*>(q_buf + (1 - half) * PP_HALF + row * 128 + lane * 4) = l;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->l_full[s][quarter]);
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->l_full[s][quarter], n_o & 1, abort_flag, p.status, 15));
+        if (!ok) break;
+        l += *reinterpret_cast<const float*>(q_buf + half * PP_HALF + row * 128 + lane * 4);
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[s], n_o & 1, abort_flag, p.status, 7));
+        if (!ok) break;
+        tc_fence_after();
+        __syncwarp();                                                // all lanes have their sums before the rows are overwritten
+        finish(item, 0.f, l, q_buf + half * PP_HALF);
+      } else {
+        float m_ref = PP_NEG, l = 0.f;
+        uint32_t r[128];
+        for (int j = jlo; j <= jhi; ++j) {
+          ok = scores_there();
+          if (!ok) break;
+#pragma unroll
+          for (int c = 0; c < 128; c += 32) tmem_ld32(s_tmem + c, r + c);
+          tc_wait_ld();
+          if (j < f_lo || j > f_hi) {
+            const int hi = q_row - j * PP_BN, lo = p.window > 0 ? hi - p.window : -1;
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+              if (!(i > lo && i <= hi)) r[i] = 0xff800000u;          // -inf
+          }
+          // the reference maximum follows the row's only when that has grown by more than 8: weights stay below 2^8
+          float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            m0 = fmax3(m0, __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+            m1 = fmax3(m1, __uint_as_float(r[32 + i]), __uint_as_float(r[33 + i]));
+            m2 = fmax3(m2, __uint_as_float(r[64 + i]), __uint_as_float(r[65 + i]));
+            m3 = fmax3(m3, __uint_as_float(r[96 + i]), __uint_as_float(r[97 + i]));
+          }
+          const float m_tgt = fmaxf(m_ref, fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * c2);
+          if (j == jlo) {
+            m_ref = m_tgt;
+          } else if (__any_sync(0xffffffffu, m_tgt - m_ref > 8.0f)) {
+            const float alpha = fast_exp2(m_ref - m_tgt);
+            m_ref = m_tgt;
+            l *= alpha;
+            uint32_t t16[16];
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              tmem_ld16(o_tmem + 16 * c, t16);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) t16[i] = __float_as_uint(__uint_as_float(t16[i]) * alpha);
+              tmem_st16(o_tmem + 16 * c, t16);
+            }
+          }
+          const uint64_t c2p = pack2f(c2, c2), nm = pack2f(-m_ref, -m_ref);
+          uint64_t sum_a = pack2f(0.f, 0.f), sum_b = sum_a;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              float x0, x1, x2, x3;
+              unpack2f(ffma2(pack2f(__uint_as_float(r[32 * c + i]), __uint_as_float(r[32 * c + i + 1])), c2p, nm), x0, x1);
+              unpack2f(ffma2(pack2f(__uint_as_float(r[32 * c + i + 2]), __uint_as_float(r[32 * c + i + 3])), c2p, nm), x2, x3);
+              const float p0 = fast_exp2(x0), p1 = fast_exp2(x1), p2 = fast_exp2(x2), p3 = fast_exp2(x3);
+              sum_a = fadd2(sum_a, pack2f(p0, p1));
+              sum_b = fadd2(sum_b, pack2f(p2, p3));
+              pk[i >> 1] = pack16<F16>(p0, p1);
+              pk[(i >> 1) + 1] = pack16<F16>(p2, p3);
+            }
+            tmem_st16(s_tmem + 16 * c, pk);
+          }
+          float a0, a1, b0, b1;
+          unpack2f(sum_a, a0, a1);
+          unpack2f(sum_b, b0, b1);
+          l += (a0 + a1) + (b0 + b1);
+          weights_done();
+        }
+        if (!ok) break;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[s], n_o & 1, abort_flag, p.status, 7));
+        if (!ok) break;
+        tc_fence_after();
+        finish(item, m_ref, l, q_buf);
+      }
+    }
+  }
+
+  // ------------------------------------------------------------------ teardown
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+}  // namespace daisy
+
+using namespace daisy;
+
+static int paged_prefill_smem() {
+  static bool done[daisy_host::MAX_DEVICES] = {};             // the attribute is per device
+  const int dev = daisy_host::device_slot();
+  if (dev < 0) return DAISY_ENODEV;
+  if (done[dev]) return DAISY_OK;
+  const auto allow = [](auto kernel) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PP_SMEM) == cudaSuccess; };
+  if (!allow(paged_prefill_kernel<2, false>) || !allow(paged_prefill_kernel<1, false>) || !allow(paged_prefill_kernel<1, true>)) return DAISY_ECUDA;
+  done[dev] = true;
+  return DAISY_OK;
+}
+
+// Workspace: the plan's head, pieces and sums.
+constexpr int PP_SLOTS_PER_SM = 4;
+struct PrefillRoom { int slots; int64_t max_pieces; size_t head, pieces, part, end; };
+static PrefillRoom prefill_room(int sms, int64_t tokens, int n_seq, int rows) {
+  PrefillRoom r;
+  r.slots = sms * PP_SLOTS_PER_SM;
+  // items, and the further pieces of those that are cut
+  r.max_pieces = tokens / rows + n_seq + r.slots;
+  r.head = 0;
+  r.pieces = r.head + 256;
+  r.part = r.pieces + ((size_t)r.max_pieces * sizeof(Piece) + 255) / 256 * 256;
+  r.end = r.part + (size_t)r.slots * PP_SLOT * sizeof(float);
+  return r;
+}
+// 128 queries an item where all items of that size find an SM: two streams pay by sharing K and V, not for latency
+static int prefill_rows(int sms, int64_t tokens, int n_seq, int Hq) { return (tokens / PP_BM + n_seq) * Hq <= sms ? PP_BM : 2 * PP_BM; }
+
+extern "C" size_t daisy_b200_paged_attend_ticket_bytes(void) {
+  int sms = daisy_host::sm_count_cached();
+  if (sms <= 0) sms = daisy_host::MAX_SMS;
+  return (size_t)sms * PP_SLOTS_PER_SM * 16 * sizeof(int);
+}
+
+extern "C" size_t daisy_b200_paged_attend_workspace_bytes(int B, int T, int n_seq, int Hq) {
+  if (B <= 0 || T <= 0 || n_seq <= 0 || Hq <= 0) return 0;
+  int sms = daisy_host::sm_count_cached();
+  if (sms <= 0) sms = daisy_host::MAX_SMS;
+  return prefill_room(sms, (int64_t)B * T, n_seq, prefill_rows(sms, (int64_t)B * T, n_seq, Hq)).end;
+}
+
+extern "C" int daisy_b200_paged_attend(const daisy_b200_pages* cache, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                                       const int32_t* lens, const int32_t* cu, int window,
+                                       void* out, int64_t o_sb, int64_t o_st, int64_t o_sh,
+                                       int B, int T, int Hq, int D, float scale, unsigned flags,
+                                       void* workspace, size_t workspace_bytes, int32_t* tickets, int* status_word, void* stream) {
+  PagedPrefillParams p = {};
+  if (const int rc = daisy_host::paged_cache(cache, D, &p.c); rc != DAISY_OK) return rc;
+  if (!q || !lens || !out || !workspace || !tickets || B <= 0 || T <= 0 || Hq <= 0 || Hq % cache->H || !(scale > 0.f)) return DAISY_EINVAL;
+  if (flags & ~(DAISY_BOUNDED_QK | DAISY_CACHE_FP16)) return DAISY_EINVAL;
+  if (B != (cu ? 1 : cache->n_seq)) return DAISY_EINVAL;
+  if (!daisy_aligned16(q) || !daisy_aligned16(out) || ((q_sb | q_st | q_sh | o_sb | o_st | o_sh) & 7) || (reinterpret_cast<uintptr_t>(lens) & 3) ||
+      (reinterpret_cast<uintptr_t>(cu) & 3) || (reinterpret_cast<uintptr_t>(tickets) & 3) || (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return DAISY_EALIGN;
+  // a zero stride on a dimension longer than 1 is a broadcast view, which the tile loads cannot express
+  if ((T > 1 && q_st <= 0) || (Hq > 1 && q_sh <= 0) || (B > 1 && q_sb <= 0)) return DAISY_EINVAL;
+  const int sms = daisy_host::sm_count_cached();
+  if (sms <= 0) return DAISY_ENODEV;
+  const int64_t tokens = (int64_t)B * T;
+  p.rows = prefill_rows(sms, tokens, cache->n_seq, Hq);
+  const PrefillRoom room = prefill_room(sms, tokens, cache->n_seq, p.rows);
+  if (workspace_bytes < room.end) return DAISY_EWORKSPACE;
+  if ((room.max_pieces + 1) * Hq >= ((int64_t)1 << 31) - 4096) return DAISY_EUNSUPPORTED;
+  if (const int rc = paged_prefill_smem(); rc != DAISY_OK) { (void)cudaGetLastError(); return rc; }
+  CUtensorMap tq, tk, tv;
+  auto sb = [](int64_t s, int64_t n) { return (uint64_t)(n == 1 ? 16 : s * 2); };
+  int rc;
+  const uint32_t box = (uint32_t)(cache->page < PP_BN ? cache->page : PP_BN);
+  if ((rc = daisy_host::make_tmap_bf16_dthb(&tq, q, D, T, Hq, B, sb(q_st, T), sb(q_sh, Hq), sb(q_sb, B), 64, PP_BM)) != DAISY_OK) return rc;
+  if ((rc = daisy_host::make_tmap_bf16_dthb(&tk, cache->k, D, cache->page, cache->H, cache->n_pages, cache->p_sr * 2, sb(cache->p_sh, cache->H),
+                                            sb(cache->p_sb, cache->n_pages), 64, box)) != DAISY_OK) return rc;
+  if ((rc = daisy_host::make_tmap_bf16_dthb(&tv, cache->v, D, cache->page, cache->H, cache->n_pages, cache->p_sr * 2, sb(cache->p_sh, cache->H),
+                                            sb(cache->p_sb, cache->n_pages), 64, box)) != DAISY_OK) return rc;
+  p.out = (__nv_bfloat16*)out; p.o_sb = o_sb; p.o_st = o_st; p.o_sh = o_sh;
+  p.lens = lens; p.cu = cu;
+  p.T = T; p.Hq = Hq; p.G = Hq / cache->H; p.window = window > 0 ? window : 0;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.status = status_word;
+  char* ws = (char*)workspace;
+  p.tickets = tickets;
+  p.head = (PlanHead*)(ws + room.head);
+  p.pieces = (Piece*)(ws + room.pieces);
+  p.part = (float*)(ws + room.part);
+  p.slots = room.slots; p.max_pieces = (int)room.max_pieces;
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool f16 = (flags & DAISY_CACHE_FP16) != 0;
+  // weights without a reference maximum reach 2^60, which float16 does not hold
+  const bool bounded = (flags & DAISY_BOUNDED_QK) && !f16 && scale * 1.4426950408889634f * (float)D <= 60.f;
+  cudaError_t e = daisy_host::launch_dependent(paged_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, p, sms);
+  if (e == cudaSuccess) {
+    if (bounded)  e = daisy_host::launch_dependent(paged_prefill_kernel<2, false>, dim3(sms), dim3(576), PP_SMEM, st, tq, tk, tv, p);
+    else if (f16) e = daisy_host::launch_dependent(paged_prefill_kernel<1, true>, dim3(sms), dim3(320), PP_SMEM, st, tq, tk, tv, p);
+    else          e = daisy_host::launch_dependent(paged_prefill_kernel<1, false>, dim3(sms), dim3(320), PP_SMEM, st, tq, tk, tv, p);
+  }
+  if (e != cudaSuccess) { (void)cudaGetLastError(); return DAISY_ECUDA; }
+  DAISY_CHECK_LAUNCH();
+  return DAISY_OK;
+}

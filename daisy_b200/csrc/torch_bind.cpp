@@ -109,7 +109,7 @@ void release_workspaces() {
   std::lock_guard<std::mutex> lock(g_mutex);
   g_pool.clear();
 }
-enum { WS_TOKEN = 0, WS_KDA_TOKEN = 1, WS_PAGED_DECODE = 2 };
+enum { WS_TOKEN = 0, WS_KDA_TOKEN = 1, WS_PAGED_DECODE = 2, WS_PAGED_ATTEND = 3 };
 
 // ------------------------------------------------------------------ decode step
 void rope_table(const Tensor& t, const char* name) {
@@ -1009,14 +1009,14 @@ int64_t paged_decode_workspace_bytes(int64_t n_seq, int64_t Hq, int64_t H) {
   return (int64_t)daisy_b200_paged_decode_workspace_bytes((int)n_seq, (int)Hq, (int)H, 128);
 }
 
-Tensor paged_decode_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens, int64_t window,
+Tensor paged_decode_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens, int64_t window_,
                          const OptTensor& cos, const OptTensor& sin, double scale, double eps, int64_t flags, const OptTensor& out_, const OptTensor& workspace,
                          const OptTensor& ve, const OptTensor& ve_gate) {
   bool f16;
   const daisy_b200_pages c = pages_of(k_pages, v_pages, table, &f16);
   c10::cuda::CUDAGuard guard(k_pages.device());
   req_tokens(q, "q", -1, k_pages); req_tokens(k, "k", c.H, k_pages); req_tokens(v, "v", c.H, k_pages);
-  const int64_t n = c.n_seq, Hq = q.size(2);
+  const int64_t n = c.n_seq, Hq = q.size(2), window = std::min<int64_t>(std::max<int64_t>(window_, 0), INT32_MAX);
   TORCH_CHECK_VALUE(q.size(0) == n && q.size(1) == 1 && k.size(0) == n && k.size(1) == 1 && v.size(0) == n && v.size(1) == 1, "q, k, v must hold one token for each of the ", n,
                     " sequences of block_table");
   TORCH_CHECK_VALUE(Hq >= 1 && Hq % c.H == 0, "query heads (", Hq, ") must be a multiple of the pages' heads (", c.H, ")");
@@ -1044,6 +1044,40 @@ Tensor paged_decode_step(const Tensor& q, const Tensor& k, const Tensor& v, cons
                                      vt.defined() ? vt.stride(0) : 0, vt.defined() ? vt.stride(2) : 0, logit, (int)Hq, 128, (float)scale, (float)eps,
                                      (unsigned)flags | (f16 ? DAISY_CACHE_FP16 : 0), ws.data_ptr(), (size_t)ws.numel(), status_ptr(k_pages), stream_of(k_pages)),
         "daisy_b200_paged_decode_step");
+  return out;
+}
+
+Tensor paged_attend(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens, int64_t window, const OptTensor& cu, double scale,
+                    const OptTensor& out_, bool bounded) {
+  bool f16;
+  const daisy_b200_pages c = pages_of(k_pages, v_pages, table, &f16);
+  c10::cuda::CUDAGuard guard(k_pages.device());
+  req(q, "q", k_pages.scalar_type());
+  TORCH_CHECK_VALUE(q.device() == k_pages.device(), "q is on ", q.device(), ", the pages are on ", k_pages.device());
+  TORCH_CHECK_VALUE(q.dim() == 4 && q.size(3) == 128, "q must be [B, T, H, 128]");
+  req_batch(q, "q", cu.has_value(), c.n_seq);
+  const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2);
+  TORCH_CHECK_VALUE(Hq >= 1 && Hq % c.H == 0, "query heads (", Hq, ") must be a multiple of the pages' heads (", c.H, ")");
+  const int32_t* len = ints_of(lens, "lens", c.n_seq, k_pages.device());
+  const int32_t* cup = cu.has_value() ? ints_of(*cu, "cu_seqlens", c.n_seq + 1, k_pages.device()) : nullptr;
+  const auto bf16 = q.options().dtype(at::kBFloat16);
+  Tensor out;
+  if (out_.has_value()) {
+    out = *out_;
+    req(out, "out");
+    TORCH_CHECK_VALUE(out.device() == q.device() && out.sizes() == q.sizes(), "out must be ", q.sizes(), " on ", q.device());
+  } else {
+    out = at::empty({B, T, Hq, 128}, bf16);
+  }
+  if (T == 0) return out;
+  checked_int(B * T, "q");
+  const Tensor ws = at::empty({(int64_t)daisy_b200_paged_attend_workspace_bytes((int)B, (int)T, c.n_seq, (int)checked_int(Hq, "q"))}, q.options().dtype(at::kByte));
+  const Tensor tickets = stream_workspace(q, WS_PAGED_ATTEND, (int64_t)daisy_b200_paged_attend_ticket_bytes());
+  check(daisy_b200_paged_attend(&c, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), len, cup, (int)std::min<int64_t>(std::max<int64_t>(window, 0), INT32_MAX), out.data_ptr(),
+                                out.stride(0), out.stride(1), out.stride(2), (int)B, (int)T, (int)Hq, 128, (float)scale,
+                                (bounded ? DAISY_BOUNDED_QK : 0) | (f16 ? DAISY_CACHE_FP16 : 0), ws.data_ptr(), (size_t)ws.numel(), (int32_t*)tickets.data_ptr(), status_ptr(q),
+                                stream_of(q)),
+        "daisy_b200_paged_attend");
   return out;
 }
 
@@ -1113,6 +1147,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_append", &paged_append, nogil());
   m.def("paged_decode_workspace_bytes", &paged_decode_workspace_bytes);
   m.def("paged_decode_step", &paged_decode_step, nogil());
+  m.def("paged_attend", &paged_attend, nogil());
   m.def("plain_bf16", &plain_bf16);
   m.def("kda_token_supported", &kda_token_supported);
   m.def("kda_token_workspace_bytes", &kda_token_workspace_bytes);

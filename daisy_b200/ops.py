@@ -455,6 +455,18 @@ def paged_decode_step(q_new, k_new, v_new, k_pages, v_pages, block_table, lens, 
                                    out, workspace, ve, ve_gate_logit)
 
 
+def paged_attend(q, k_pages, v_pages, block_table, lens, window: Optional[int], cu_seqlens: Optional[torch.Tensor] = None,
+                 scale: float = ATTN_SCALE, out: Optional[torch.Tensor] = None, bounded_qk: bool = False):
+    """Causal attention of a chunk of every sequence over a paged cache that holds the chunk's keys and values already
+    (:func:`paged_append`, whose returned queries this takes): ``q`` prepared, in the pages' type, ``[n, T, Hq, 128]`` or packed
+    ``[1, T_total, Hq, 128]`` with ``cu_seqlens``.  ``lens`` int32 ``[n]`` on the device: tokens of each sequence with its chunk;
+    a sequence's queries are its last ones.  Each sees the nearest ``window`` keys up to its own (None: all).  Rows of idle
+    sequences (``lens`` negative) and of sequences that hold fewer tokens than the chunk are zero (the latter show up in
+    :func:`check_device_status`), rows past ``cu_seqlens[n]`` are not written.  ``bounded_qk`` as in :func:`swa_attend`
+    (bf16 pages).  Returns bf16 of ``q``'s shape."""
+    return ext().paged_attend(q, k_pages, v_pages, block_table, lens, int(window or 0), cu_seqlens, scale, out, bounded_qk)
+
+
 def kda_chunk_fwd(q, k, v, g, beta, scale: Optional[float] = None, initial_state=None,
                   output_final_state: bool = False, l2norm_qk: bool = True, out_fp32: bool = False):
     """KDA chunked forward.  ``q,k [B,T,H,K]`` ``v [B,T,H,V]`` bf16; ``g [B,T,H,K]`` fp32 log-decay; ``beta
