@@ -255,6 +255,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     // ------------------------------------------------------------------ TMA producer: the warp as one, lane 0 issues
     if (lane == 0) { prefetch_tmap(&tm_q); prefetch_tmap(&tm_k); prefetch_tmap(&tm_v); }
     const int n_work = __ldcg(&p.head->n_pieces) * p.Hq;            // L2: this grid was there before the plan was written
+    const int lgr = min(p.c.lg, 7), boxes = PP_BN >> lgr;           // a tile is `boxes` boxes of 1 << lgr rows
     int n = 0;
     uint32_t qn[2] = {0, 0};
     bool ok = true;
@@ -322,53 +323,39 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     publish(0, g);
     if (ok && g.b >= 0) load_q(g);
     for (int rd = 0; ok && g.b >= 0; ++rd, g = g_next) {
-      // the table's entries, 32 at a time, the next 32 on their way
+      // the table's entries, a lane each, 32 at a time, the next 32 on their way
       const int* table = p.c.table + g.b * p.c.table_sb;
-      const int e_first = g.see0 >> p.c.lg, e_last = (g.end - 1) >> p.c.lg;
+      const int e_first = g.see0 >> p.c.lg, e_last = (g.end - 1) >> p.c.lg, hk = g.h / p.G;
       auto entries = [&](int from) {
         const int i = from + lane;
         return i >= e_first && i <= e_last ? __ldcg(table + i) : 0;
       };
-      int from = max((g.jlo * PP_BN) >> p.c.lg, 0);
-      int cur = 0, ahead = 0;
-      if (g.jhi >= g.jlo) { cur = entries(from); ahead = entries(from + 32); }
-      auto page_of = [&](int e) {                                    // e not below `from`
-        while (e >= from + 32) { from += 32; cur = ahead; ahead = entries(from + 32); }
-        int pg = __shfl_sync(0xffffffffu, cur, e - from);
-        if ((unsigned)pg >= (unsigned)p.c.n_pages) {
-          if (p.status && lane == 0) p.status[0] = DAISY_EINVAL;
-          pg = 0;
-        }
-        return pg;
-      };
+      int from = 0, cur = 0, ahead = 0;
+      if (g.jhi >= g.jlo) { from = (g.jlo * PP_BN) >> p.c.lg; cur = entries(from); ahead = entries(from + 32); }
       bool next_out = false;
       for (int j = g.jlo; j <= g.jhi && ok; ++j) {
-        const int rows = min(1 << p.c.lg, PP_BN), boxes = PP_BN / rows;
-        const int k0 = j * PP_BN;
-        // boxes that hold a row somebody sees
-        const int b_first = max(g.see0 - k0, 0) / rows, b_last = (min(g.end - k0, PP_BN) - 1) / rows;
-        int pages[8];
-        const int e_lo = k0 >> p.c.lg;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          pages[i] = 0;
-          if (i < boxes && i >= b_first && i <= b_last) pages[i] = page_of(e_lo + (rows < PP_BN ? i : 0));
+        // a lane a box (32 is a multiple of the boxes of a tile); only those that hold a row somebody sees
+        const int k0 = j * PP_BN, e_lo = k0 >> p.c.lg;
+        if (e_lo >= from + 32) { from += 32; cur = ahead; ahead = entries(from + 32); }
+        int pg = __shfl_sync(0xffffffffu, cur, e_lo - from + (lane & (boxes - 1)));
+        const int b_first = max(g.see0 - k0, 0) >> lgr, b_last = (min(g.end - k0, PP_BN) - 1) >> lgr;
+        const bool mine = lane >= b_first && lane <= b_last;
+        if (mine && (unsigned)pg >= (unsigned)p.c.n_pages) {
+          if (p.status) p.status[0] = DAISY_EINVAL;
+          pg = 0;
         }
-        const uint32_t bytes = (uint32_t)(b_last - b_first + 1) * rows * 256u;
+        const uint32_t bytes = (uint32_t)(b_last - b_first + 1) << (lgr + 8);
+        const int in_page = k0 & ((1 << p.c.lg) - 1);                // of a page longer than a tile
         for (int kv = 0; kv < 2; ++kv, ++n) {
           const int stage = n % PP_NSTAGE;
           if (!wait(&bars->kv_empty[stage], ((n / PP_NSTAGE) & 1) ^ 1, 1)) { ok = false; break; }
-          if (lane == 0) {
-            uint8_t* dst = kv_tiles + stage * PP_TILE;
+          if (lane == 0) mbar_expect_tx(&bars->kv_full[stage], bytes);
+          __syncwarp();
+          if (mine) {
+            uint8_t* dst = kv_tiles + stage * PP_TILE + (lane << (lgr + 7));
             const CUtensorMap* tm = kv ? &tm_v : &tm_k;
-            mbar_expect_tx(&bars->kv_full[stage], bytes);
-            const int in_page = k0 & ((1 << p.c.lg) - 1);            // of a page longer than a tile
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (i >= b_first && i <= b_last) {
-                tma_load_4d(dst + i * rows * 128, tm, &bars->kv_full[stage], 0, in_page, g.h / p.G, pages[i]);
-                tma_load_4d(dst + PP_HALF + i * rows * 128, tm, &bars->kv_full[stage], 64, in_page, g.h / p.G, pages[i]);
-              }
+            tma_load_4d(dst, tm, &bars->kv_full[stage], 0, in_page, hk, pg);
+            tma_load_4d(dst + PP_HALF, tm, &bars->kv_full[stage], 64, in_page, hk, pg);
           }
           __syncwarp();
         }
