@@ -1,7 +1,9 @@
 // One new token of every sequence against a paged cache: the work of a batch of uneven lengths dealt out in equal shares, one launch.
 //
-// Bound by HBM: 512 bytes for every cached row and key head, read once for all query heads of the group.  The cached rows
-// of all (sequence, key head) pairs lie end to end in tiles of 16; every CTA takes an equal run of tiles, whatever sequences it
+// Bound by HBM: 512 bytes for every cached row and key head, read once for all query heads of the group (64 sequences x 4096 rows x 16
+// heads 321 us, 6.7 TB/s; 1 x 131071 x 16 167 us; 24 of up to 16384 rows, 32 query heads over 8, 135 us; 1 x 511 rows x 6 8.4 us, four
+// of them the chain length -> page -> rows and the join).  The cached rows
+// of all (sequence, key head) pairs lie end to end in blocks of four 16-row tiles; every CTA takes an equal run of blocks, whatever sequences it
 // cuts, so neither uneven lengths nor a wide block table leaves an SM idle (the host knows no lengths).  A pair that
 // several CTAs share is joined by the last of them, from partial sums in a fixed order: the same bits every run.  That last one,
 // or the only one, also prepares the token's own row, adds it and stores it.
@@ -31,22 +33,28 @@ struct PagedDecodeParams {
   unsigned flags;
   int* status;
   float* part;                       // [2 grid][8 NT][PD_PART]: 128 sums, reference, denominator
-  int* tickets;                      // [n_seq H n_grp], zero between calls
+  int *tickets, *tickets_grp;        // [n_seq H n_grp], [2 grid], zero between calls
 };
 constexpr int PD_PART = 132;
+// What a pair costs beside its rows (queries, sums of the warps, the token's own row, output), in blocks of 64 rows: the deal counts it
+// as so many blocks without rows in front of the pair's.
+constexpr int PD_HEAD = 2;
+constexpr int PD_JOIN = 16;          // shares that one CTA joins
 constexpr __host__ __device__ int pd_ctas(int cols) { return cols == 8 ? 3 : 2; }              // CTAs a SM, by registers
 
 // Where a sequence stands: its cached length, or -1 if it is idle or cannot have the position; rows lo .. len-1 are seen.
-struct SeqRange { int len, lo, tile0, tiles; };
-__device__ __forceinline__ SeqRange seq_range(const PagedDecodeParams& p, int b) {
+struct SeqRange { int len, lo, tile0, tiles, blocks; };              // blocks: PD_HEAD, then one for every PD_WARPS tiles, the last one maybe short
+__device__ __forceinline__ int seq_len(const PagedDecodeParams& p, int b) { return __ldcg(p.lens + b); }   // L2: this grid may have been there before they were written
+__device__ __forceinline__ SeqRange seq_range(const PagedDecodeParams& p, int len) {
   SeqRange r;
-  r.len = __ldcg(p.lens + b);                                        // L2: this grid may have been there before they were written
+  r.len = len;
   const bool bad = r.len >= p.c.capacity() || ((p.flags & DAISY_ROPE) && r.len >= p.table_rows);
   if (bad && p.status) p.status[0] = DAISY_EINVAL;
   if (r.len < 0 || bad) r.len = -1;
   r.lo = p.window > 0 && r.len > p.window - 1 ? r.len - (p.window - 1) : 0;
   r.tile0 = r.lo / PD_TILE;
   r.tiles = r.len <= r.lo ? 1 : (r.len + PD_TILE - 1) / PD_TILE - r.tile0;      // one without rows: the token alone
+  r.blocks = PD_HEAD + (r.tiles + PD_WARPS - 1) / PD_WARPS;
   return r;
 }
 
@@ -92,85 +100,274 @@ __device__ __forceinline__ void row_of_warp(const __nv_bfloat16* src, bool norm,
   }
 }
 
-// Sum over all sequences of their tiles; with `want` >= 0 also the sequence that holds tile `want` of the batch (tiles of one head)
-// and the tiles in front of it.  The whole block calls it.
-struct Found { int64_t total; int b; int64_t before; };
-__device__ __forceinline__ Found scan_tiles(const PagedDecodeParams& p, int64_t want, int64_t* sm) {
-  Found f{0, -1, 0};
+// Lengths of the first PD_KEPT sequences stay in shared memory.
+constexpr int PD_KEPT = 32 * PD_WARPS;
+struct DealSmem { int warp_sum[PD_WARPS]; int before, b; int len[PD_KEPT]; };
+
+// This CTA's run of blocks [t, t_end) of the batch, the sequence b that holds t, and where b's blocks begin.  The whole block calls it.
+struct Deal { int t, t_end, share, b_at, b; };
+__device__ __forceinline__ Deal deal_tiles(const PagedDecodeParams& p, int HH, DealSmem* sm) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int b0 = 0; b0 < p.c.n_seq; b0 += 32 * PD_WARPS) {
+  Deal d;
+  int base, x, t, total = 0;
+  // blocks (of one head) of sequences b0 .. b0 + PD_KEPT - 1: this thread's, their inclusive prefix sum, what lies in front of its warp
+  auto scan = [&](int b0) {
     const int b = b0 + threadIdx.x;
-    const int64_t t = b < p.c.n_seq ? seq_range(p, b).tiles : 0;
-    int64_t x = t;
+    const int len = b < p.c.n_seq ? seq_len(p, b) : -1;
+    if (b0 == 0) sm->len[threadIdx.x] = len;
+    x = t = b < p.c.n_seq ? seq_range(p, len).blocks : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
+    if (lane == 31) sm->warp_sum[warp] = x;
     __syncthreads();
-    if (lane == 31) sm[warp] = x;
-    if (threadIdx.x == 0) sm[PD_WARPS] = -1;
+    base = 0;
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < PD_WARPS; ++w) { if (w < warp) base += sm->warp_sum[w]; sum += sm->warp_sum[w]; }
+    return sum;
+  };
+  if (threadIdx.x == 0) sm->b = -1;
+  total = scan(0);
+  const int first_sum = total;
+  for (int b0 = PD_KEPT; b0 < p.c.n_seq; b0 += PD_KEPT) {
     __syncthreads();
-    int64_t base = f.total, sum = 0;
-    for (int w = 0; w < PD_WARPS; ++w) { if (w < warp) base += sm[w]; sum += sm[w]; }
-    if (want >= 0 && t > 0 && base + x - t <= want && want < base + x) { sm[PD_WARPS] = b; sm[PD_WARPS + 1] = base + x - t; }
-    __syncthreads();
-    if (want >= 0 && sm[PD_WARPS] >= 0) { f.b = (int)sm[PD_WARPS]; f.before = sm[PD_WARPS + 1]; return f; }
-    f.total += sum;
+    total += scan(b0);
   }
-  return f;
+  total *= HH;
+  d.share = (int)(((unsigned)total + gridDim.x - 1) / gridDim.x);
+  d.t = min((unsigned)blockIdx.x * (unsigned)d.share, (unsigned)total);
+  d.t_end = (int)min((unsigned)d.t + (unsigned)d.share, (unsigned)total);
+  d.b = -1;
+  if (d.t >= d.t_end) return d;
+  const int want = d.t / HH;
+  int front = 0;
+  for (int b0 = 0; b0 < p.c.n_seq; b0 += PD_KEPT) {
+    int sum = first_sum;
+    if (p.c.n_seq > PD_KEPT) { __syncthreads(); sum = scan(b0); }
+    if (want < front + sum) {
+      const int at = front + base + x - t;
+      if (t > 0 && at <= want && want < at + t) { sm->b = b0 + threadIdx.x; sm->before = at; }
+      break;
+    }
+    front += sum;
+  }
+  __syncthreads();
+  d.b = sm->b;
+  d.b_at = sm->before * HH;
+  return d;
+}
+
+// Sums of one head: channels 4 lane .. of the numerator, reference, denominator.
+struct Sums { float4 num; float ref, den; };
+
+// Shares of CTAs from, from + step, .. <= to, every fourth to a warp, into the warps' places in shared memory (acc [4][NQ][128], m, l [4][NQ]).
+// A function of its own: inlined, what it computes ahead takes the registers of the main loop (spills, 322 -> 458 us); with four heads at once
+// its own registers do (322 -> 550 us).
+template <int NQ>
+__device__ __noinline__ void join_shares(const float* part, float* acc, float* m, float* l, int n_q, int from, int to, int step, int first_cta) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int col = 0; col < n_q; col += 2) {
+    Sums x[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) x[k] = Sums{make_float4(0.f, 0.f, 0.f, 0.f), PD_NEG, 0.f};
+    for (int cc = from + warp * step; cc <= to; cc += 4 * PD_WARPS * step) {
+      float4 n1[4][2];
+      float2 rd[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int ci = cc + i * PD_WARPS * step <= to ? cc + i * PD_WARPS * step : cc;
+        const float* src = part + ((int64_t)ci * 2 + (ci == first_cta ? 1 : 0)) * NQ * PD_PART + col * PD_PART;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (k == 0 || col + 1 < n_q) {
+            n1[i][k] = __ldcg(reinterpret_cast<const float4*>(src + k * PD_PART) + lane);
+            rd[i][k] = __ldcg(reinterpret_cast<const float2*>(src + k * PD_PART + 128));
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (cc + i * PD_WARPS * step <= to) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (k == 0 || col + 1 < n_q) {
+              Sums& y = x[k];
+              const float top = fmaxf(y.ref, rd[i][k].x), a = fast_exp2(y.ref - top), e = fast_exp2(rd[i][k].x - top);
+              y.num = make_float4(y.num.x * a + e * n1[i][k].x, y.num.y * a + e * n1[i][k].y, y.num.z * a + e * n1[i][k].z, y.num.w * a + e * n1[i][k].w);
+              y.den = y.den * a + e * rd[i][k].y;
+              y.ref = top;
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (k == 0 || col + 1 < n_q) {
+        *reinterpret_cast<float4*>(acc + (warp * NQ + col + k) * DAISY_HEAD_DIM + 4 * lane) = x[k].num;
+        if (lane == 0) { m[warp * NQ + col + k] = x[k].ref; l[warp * NQ + col + k] = x[k].den; }
+      }
+  }
+}
+
+// The token's own row of pair (b, h) and its scores, by all warps but the first: k and v as they will lie in the page, its page, v in fp32, the
+// scores of query heads q_h0 .. q_h0 + n_q - 1 (in the exp2 domain).
+struct OwnRow { float4 v[32]; uint2 k16[32], v16[32]; int page; };
+template <bool F16>
+__device__ __forceinline__ void own_row(const PagedDecodeParams& p, int b, int h, int q_h0, int n_q, int len, OwnRow* own, float* scores) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float *cos_row = p.cos + (int64_t)len * 64, *sin_row = p.sin + (int64_t)len * 64;
+  int page = 0;
+  if (warp == PD_WARPS - 1) page = __ldcg(p.c.table + b * p.c.table_sb + (len >> p.c.lg));
+  float kr[4];
+  row_of_warp(p.k + b * p.k_sb + h * p.k_sh, p.flags & DAISY_NORM_K, p.flags & DAISY_ROPE, p.eps, cos_row, sin_row, lane, kr);
+  const uint2 k16 = make_uint2(pack16<F16>(kr[0], kr[1]), pack16<F16>(kr[2], kr[3]));
+  const float2 ka = unpack16<F16>(k16.x), kc = unpack16<F16>(k16.y);
+  for (int col = warp - 1; col < n_q; col += PD_WARPS - 1) {
+    float x[4];
+    row_of_warp(p.q + b * p.q_sb + (q_h0 + col) * p.q_sh, p.flags & DAISY_NORM_Q, p.flags & DAISY_ROPE, p.eps, cos_row, sin_row, lane, x);
+    const float s = warp_sum(x[0] * ka.x + x[1] * ka.y + x[2] * kc.x + x[3] * kc.y) * p.qscale;
+    if (lane == 0) scores[col] = s;
+  }
+  if (warp == PD_WARPS - 1) {
+    float vr[4];
+    row_of_warp(p.v + b * p.v_sb + h * p.v_sh, p.flags & DAISY_NORM_V, false, p.eps, cos_row, sin_row, lane, vr);
+    if (p.ve) {
+      const float gate = 1.0f / (1.0f + __expf(-*p.ve_gate));
+      const uint2 u = *reinterpret_cast<const uint2*>(p.ve + b * p.ve_sb + h * p.ve_sh + 4 * lane);
+      const float e[4] = {bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vr[i] = gate * vr[i] + (1.0f - gate) * e[i];
+    }
+    const uint2 v16 = make_uint2(pack16<F16>(vr[0], vr[1]), pack16<F16>(vr[2], vr[3]));
+    const float2 va = unpack16<F16>(v16.x), vc = unpack16<F16>(v16.y);
+    own->v[lane] = make_float4(va.x, va.y, vc.x, vc.y);
+    own->k16[lane] = k16;
+    own->v16[lane] = v16;
+    if (lane == 0) own->page = page;
+  }
 }
 
 template <int NT, bool F16>
-__global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_kernel(const PagedDecodeParams p) {
+__global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
   constexpr int NQ = 8 * NT;                                         // query heads of a pass, the last ones maybe absent
-  __shared__ int64_t sm_scan[PD_WARPS + 2];
+  __shared__ DealSmem sm_deal;
   __shared__ __align__(16) float sm_acc[PD_WARPS][NQ][DAISY_HEAD_DIM];
   __shared__ float sm_m[PD_WARPS][NQ], sm_l[PD_WARPS][NQ];
   __shared__ float sm_self[NQ];
-  __shared__ __align__(16) float sm_v[DAISY_HEAD_DIM];
+  __shared__ OwnRow sm_own;
   __shared__ int sm_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int HH = p.c.H * p.n_grp;                                    // pairs a sequence
   grid_dep_launch();
   grid_dep_wait();
 
-  const int64_t total = scan_tiles(p, -1, sm_scan).total * HH;
-  int64_t share = (total + gridDim.x - 1) / gridDim.x;
-  share = (share + PD_WARPS - 1) / PD_WARPS * PD_WARPS;
-  int64_t t = (int64_t)blockIdx.x * share;
-  const int64_t t_end = min(t + share, total);
-  if (t >= t_end) return;
-  const Found f = scan_tiles(p, t / HH, sm_scan);                    // pairs are (sequence, head)-major: head h of b begins at before HH + h tiles
-  int b = f.b;
-  if (b < 0) return;
-  int64_t b_at = f.before * HH;
-  SeqRange r = seq_range(p, b);
+  const Deal deal = deal_tiles(p, HH, &sm_deal);                     // pairs are (sequence, head)-major
+  if (deal.b < 0) return;
+  const int t_end = deal.t_end, share = deal.share;
+  int t = deal.t, b_at = deal.b_at;
+  int b = deal.b;
+  auto range_of = [&](int i) { return seq_range(p, i < PD_KEPT ? sm_deal.len[i] : seq_len(p, i)); };
+  SeqRange r = range_of(b);
 
   while (t < t_end) {
-    while (t >= b_at + (int64_t)r.tiles * HH) {
+    while (t >= b_at + r.blocks * HH) {
       if (b + 1 >= p.c.n_seq) return;                                // lengths that changed under the call
-      b_at += (int64_t)r.tiles * HH;
-      r = seq_range(p, ++b);
+      b_at += r.blocks * HH;
+      r = range_of(++b);
     }
-    const int hh = (int)((t - b_at) / r.tiles), h = hh / p.n_grp, grp = hh % p.n_grp;
-    const int64_t u_at = b_at + (int64_t)hh * r.tiles;               // this pair's tiles: u_at .. u_end - 1
-    const int64_t u_end = u_at + r.tiles, s_end = min(u_end, t_end);
+    const int hh = (t - b_at) / r.blocks, h = hh / p.n_grp, grp = hh % p.n_grp;
+    const int u_at = b_at + hh * r.blocks;                           // this pair's blocks: u_at .. u_end - 1
+    const int u_end = u_at + r.blocks, s_end = min(u_end, t_end);
+    const int r_at = max(t, u_at + PD_HEAD);                         // this CTA's blocks with rows: r_at .. s_end - 1
+    if (r_at >= s_end) { t = s_end; continue; }
     const int q_h0 = h * p.G + grp * NQ, n_q = min(NQ, p.G - grp * NQ);
     const float *cos_row = p.cos + (int64_t)max(r.len, 0) * 64, *sin_row = p.sin + (int64_t)max(r.len, 0) * 64;
 
+    // what the queries are made of is asked for first: the table's entry and the rows behind it take longer
+    uint4 q_raw[NT][4];
+    float4 cs4[2][2], sn4[2][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        q_raw[n][j] = 8 * n + g < n_q ? ld_cg16(p.q + b * p.q_sb + (q_h0 + 8 * n + g) * p.q_sh + 32 * j + 8 * c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        cs4[j][i] = make_float4(1.f, 1.f, 1.f, 1.f);
+        sn4[j][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p.flags & DAISY_ROPE) {
+          cs4[j][i] = *reinterpret_cast<const float4*>(cos_row + 32 * j + 8 * c + 4 * i);
+          sn4[j][i] = *reinterpret_cast<const float4*>(sin_row + 32 * j + 8 * c + 4 * i);
+        }
+      }
+    const int* table = p.c.table + b * p.c.table_sb;
+    const int first = r.tile0 + (r_at - u_at - PD_HEAD) * PD_WARPS, last = r.tile0 + min((s_end - u_at - PD_HEAD) * PD_WARPS, r.tiles);    // tiles of the sequence
+    auto page_of = [&](int tile) -> int {                            // a row outside the pool is taken from page 0
+      int pg = tile < last && r.len > r.lo ? __ldcg(table + ((tile * PD_TILE) >> p.c.lg)) : 0;
+      if ((unsigned)pg >= (unsigned)p.c.n_pages) {
+        if (p.status) p.status[0] = DAISY_EINVAL;
+        pg = 0;
+      }
+      return pg;
+    };
+    // A tile's rows as lane (g, c) takes them: keys g, g + 8, pieces 32 j + 8 c of the channels; values of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9, channels
+    // 8 g .. and 64 + 8 g ...  Rows that nobody sees may hold anything: they count as zeros.
+    const int64_t sr = 2 * p.c.p_sr;
+    auto seen = [&](int row) { return row >= r.lo && row < r.len; };
+    auto whole = [&](int tile) { return tile * PD_TILE >= r.lo && tile * PD_TILE + PD_TILE <= r.len; };
+    auto fetch_k = [&](int tile, int pg, uint4 (&kk)[2][4]) {
+      const char* kb = p.c.k + p.c.at(pg, h, tile * PD_TILE) + 16 * c;
+      if (whole(tile)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) kk[i][j] = ld_stream16(kb + (g + 8 * i) * sr + 64 * j);
+        return;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool in = seen(tile * PD_TILE + g + 8 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kk[i][j] = in ? ld_stream16(kb + (g + 8 * i) * sr + 64 * j) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto fetch_v = [&](int tile, int pg, uint4 (&vv)[4][2]) {
+      const char* vb = p.c.v + p.c.at(pg, h, tile * PD_TILE) + 16 * g;
+      if (whole(tile)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) vv[i][j] = ld_stream16(vb + (2 * c + (i & 1) + 8 * (i >> 1)) * sr + 128 * j);
+        return;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 2 * c + (i & 1) + 8 * (i >> 1);
+        const bool in = seen(tile * PD_TILE + row);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) vv[i][j] = in ? ld_stream16(vb + row * sr + 128 * j) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    uint4 kk[2][4], vv[4][2];
+    int pg = page_of(first + warp), pg_next = page_of(first + warp + PD_WARPS);
+    if (first + warp < last) {                                       // on their way under the queries' preparation
+      fetch_k(first + warp, pg, kk);
+      fetch_v(first + warp, pg, vv);
+    }
     // ---------------------------------------------------------------- the queries as B operands: lane (g, c) holds head 8 n + g, channels
     // 32 j + 8 c .. + 7 for j = 0..3; element pair i of piece j goes to k step 2 j + i / 2
-    uint32_t qh[NT][4][4], ql[NT][4][4];
+    // The second halves of the sums lie in shared memory, a lane's own (16 registers NT that the rows' loads need); the place is the warp's sums',
+    // which are left there after the last tile.
+    uint32_t qh[NT][4][4];
+    uint4* q_low = reinterpret_cast<uint4*>(&sm_acc[warp][0][0]) + lane;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float x[4][8];
-      const bool live = 8 * n + g < n_q;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint4 u = live ? ld_cg16(p.q + b * p.q_sb + (q_h0 + 8 * n + g) * p.q_sh + 32 * j + 8 * c) : make_uint4(0, 0, 0, 0);
-        unpack8(u, x[j]);
-      }
+      for (int j = 0; j < 4; ++j) unpack8(q_raw[n][j], x[j]);
       float mul = p.qscale;
       if (p.flags & DAISY_NORM_Q) {
         float ss = 0.f;
@@ -183,23 +380,28 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
         mul *= rsqrtf(ss * (1.0f / DAISY_HEAD_DIM) + p.eps);
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j) {
+        const float cs[8] = {cs4[j][0].x, cs4[j][0].y, cs4[j][0].z, cs4[j][0].w, cs4[j][1].x, cs4[j][1].y, cs4[j][1].z, cs4[j][1].w};
+        const float sn[8] = {sn4[j][0].x, sn4[j][0].y, sn4[j][0].z, sn4[j][0].w, sn4[j][1].x, sn4[j][1].y, sn4[j][1].z, sn4[j][1].w};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          float cs = 1.f, sn = 0.f;
-          if (p.flags & DAISY_ROPE) { cs = cos_row[32 * j + 8 * c + e]; sn = sin_row[32 * j + 8 * c + e]; }
           const float a = x[j][e] * mul, d = x[j + 2][e] * mul;
-          x[j][e] = a * cs + d * sn;
-          x[j + 2][e] = d * cs - a * sn;
+          x[j][e] = a * cs[e] + d * sn[e];
+          x[j + 2][e] = d * cs[e] - a * sn[e];
         }
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
+      {
+        uint32_t lo[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           qh[n][j][i] = pack16<F16>(x[j][2 * i], x[j][2 * i + 1]);
           const float2 back = unpack16<F16>(qh[n][j][i]);
-          ql[n][j][i] = pack16<F16>(x[j][2 * i] - back.x, x[j][2 * i + 1] - back.y);
+          lo[i] = pack16<F16>(x[j][2 * i] - back.x, x[j][2 * i + 1] - back.y);
         }
+        q_low[(n * 4 + j) * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
     }
 
     float acc[NT][8][4];                                             // channels 8 g + e (elements 0, 1) and 64 + 8 g + e of heads 2 c, 2 c + 1
@@ -212,65 +414,28 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
       l[n][0] = l[n][1] = 0.f;
     }
 
-    const int* table = p.c.table + b * p.c.table_sb;
-    const int first = r.tile0 + (int)(t - u_at), last = r.tile0 + (int)(s_end - u_at);    // tiles of the sequence
-    auto page_of = [&](int tile) -> int {                            // a row outside the pool is taken from page 0
-      int pg = tile < last && r.len > r.lo ? __ldcg(table + ((tile * PD_TILE) >> p.c.lg)) : 0;
-      if ((unsigned)pg >= (unsigned)p.c.n_pages) {
-        if (p.status) p.status[0] = DAISY_EINVAL;
-        pg = 0;
-      }
-      return pg;
-    };
-    int pg = page_of(first + warp);
     for (int tile = first + warp; tile < last; tile += PD_WARPS) {
-      const int row0 = tile * PD_TILE;
-      const char *kb = p.c.k + p.c.at(pg, h, row0) + 16 * c, *vb = p.c.v + p.c.at(pg, h, row0) + 16 * g;
-      const int64_t sr = 2 * p.c.p_sr;
-      const bool whole = row0 >= r.lo && row0 + PD_TILE <= r.len;
-      uint4 kk[2][4], vv[4][2];
-      if (whole) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) kk[i][j] = ld_stream16(kb + (g + 8 * i) * sr + 64 * j);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) vv[i][j] = ld_stream16(vb + (2 * c + (i & 1) + 8 * (i >> 1)) * sr + 128 * j);
-      } else {                                                       // rows that nobody sees may hold anything: they count as zeros
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = g + 8 * i;
-          const bool in = row0 + row >= r.lo && row0 + row < r.len;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) kk[i][j] = in ? ld_stream16(kb + row * sr + 64 * j) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = 2 * c + (i & 1) + 8 * (i >> 1);
-          const bool in = row0 + row >= r.lo && row0 + row < r.len;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) vv[i][j] = in ? ld_stream16(vb + row * sr + 128 * j) : make_uint4(0, 0, 0, 0);
-        }
-      }
-      pg = page_of(tile + PD_WARPS);
+      const int row0 = tile * PD_TILE, next = tile + PD_WARPS;
+      if (tile != first + warp) { fetch_k(tile, pg_next, kk); fetch_v(tile, pg_next, vv); pg_next = page_of(next); }
       float s[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
+        uint4 ql[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) ql[n] = q_low[(n * 4 + j) * 32];
         const uint32_t k0[4] = {kk[0][j].x, kk[0][j].y, kk[0][j].z, kk[0][j].w}, k1[4] = {kk[1][j].x, kk[1][j].y, kk[1][j].z, kk[1][j].w};
 #pragma unroll
         for (int i = 0; i < 4; i += 2)
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             mma16816<F16>(s[n], k0[i], k1[i], k0[i + 1], k1[i + 1], qh[n][j][i], qh[n][j][i + 1]);
-            mma16816<F16>(s[n], k0[i], k1[i], k0[i + 1], k1[i + 1], ql[n][j][i], ql[n][j][i + 1]);
+            mma16816<F16>(s[n], k0[i], k1[i], k0[i + 1], k1[i + 1], i ? ql[n].z : ql[n].x, i ? ql[n].w : ql[n].y);
           }
       }
-      if (!whole) {
-        const bool in0 = row0 + g >= r.lo && row0 + g < r.len, in1 = row0 + g + 8 >= r.lo && row0 + g + 8 < r.len;
+      if (!whole(tile)) {
+        const bool in0 = seen(row0 + g), in1 = seen(row0 + g + 8);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           if (!in0) s[n][0] = s[n][1] = -INFINITY;
@@ -321,6 +486,7 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
     }
 
     // ---------------------------------------------------------------- the four warps' sums
+    __syncwarp();
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -340,99 +506,96 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
         }
       }
     __syncthreads();
-    const int d = threadIdx.x;
-    const bool alone = u_at >= (int64_t)blockIdx.x * share && u_end <= t_end;
-    // this CTA's sums of head `col`: numerator of channel d, reference, denominator
-    auto mine = [&](int col, float& num, float& ref, float& den) {
-      ref = fmaxf(fmaxf(sm_m[0][col], sm_m[1][col]), fmaxf(sm_m[2][col], sm_m[3][col]));
-      num = den = 0.f;
+    const bool alone = u_at + PD_HEAD >= deal.t && u_end <= t_end;
+    // sums of head `col` over the four warps
+    auto mine = [&](int col) {
+      Sums x{make_float4(0.f, 0.f, 0.f, 0.f), fmaxf(fmaxf(sm_m[0][col], sm_m[1][col]), fmaxf(sm_m[2][col], sm_m[3][col])), 0.f};
 #pragma unroll
       for (int w = 0; w < PD_WARPS; ++w) {
-        const float s = fast_exp2(sm_m[w][col] - ref);
-        num = fmaf(s, sm_acc[w][col][d], num);
-        den = fmaf(s, sm_l[w][col], den);
+        const float e = fast_exp2(sm_m[w][col] - x.ref);
+        const float4 y = *reinterpret_cast<const float4*>(&sm_acc[w][col][4 * lane]);
+        x.num.x = fmaf(e, y.x, x.num.x); x.num.y = fmaf(e, y.y, x.num.y); x.num.z = fmaf(e, y.z, x.num.z); x.num.w = fmaf(e, y.w, x.num.w);
+        x.den = fmaf(e, sm_l[w][col], x.den);
       }
+      return x;
     };
-    bool finish = alone;
-    const int64_t c0 = u_at / share, c1 = (u_end - 1) / share;        // the CTAs that share this pair
+    const int c0 = (u_at + PD_HEAD) / share, c1 = (u_end - 1) / share;            // the CTAs that share this pair
+    // Shares are joined by groups of PD_JOIN CTAs, then the groups: the last one of a group to come joins it into the place of the
+    // group's first, the last group the pair.
+    const int c_grp = c0 + ((int)blockIdx.x - c0) / PD_JOIN * PD_JOIN, n_grps = (c1 - c0) / PD_JOIN + 1;
+    auto place = [&](int cta) { return (int64_t)cta * 2 + (cta == c0 ? 1 : 0); };
     if (!alone) {
-      float* dst = p.part + ((int64_t)blockIdx.x * 2 + (blockIdx.x == c0 ? 1 : 0)) * NQ * PD_PART;
-      for (int col = 0; col < n_q; ++col) {
-        float num, ref, den;
-        mine(col, num, ref, den);
-        dst[col * PD_PART + d] = num;
-        if (d == 0) { dst[col * PD_PART + 128] = ref; dst[col * PD_PART + 129] = den; }
+      float* dst = p.part + place(blockIdx.x) * NQ * PD_PART;
+      for (int col = warp; col < n_q; col += PD_WARPS) {
+        const Sums x = mine(col);
+        __stcg(reinterpret_cast<float4*>(dst + col * PD_PART) + lane, x.num);
+        if (lane == 0) __stcg(reinterpret_cast<float2*>(dst + col * PD_PART + 128), make_float2(x.ref, x.den));
+      }
+      __threadfence();
+      __syncthreads();
+    }
+    // one thread asks whether all other shares are there; under that the other warps prepare the token's own row
+    if (threadIdx.x == 0) {
+      sm_last = 1;
+      if (!alone) {                                                  // of the group's shares, or of the pair's where there is one group
+        int* tk = n_grps > 1 ? p.tickets_grp + place(c_grp) : p.tickets + ((int64_t)b * HH + hh);
+        const int of = min(c_grp + PD_JOIN - 1, c1) - c_grp;
+        sm_last = atomicAdd(tk, 1) == of;
+        if (sm_last) *tk = 0;                                        // every other one has been drawn
+      }
+    } else if (warp > 0 && r.len >= 0) {
+      own_row<F16>(p, b, h, q_h0, n_q, r.len, &sm_own, sm_self);
+    }
+    __syncthreads();
+    bool finish = sm_last != 0;
+    if (finish && !alone) {
+      __threadfence();
+      join_shares<NQ>(p.part, &sm_acc[0][0][0], &sm_m[0][0], &sm_l[0][0], n_q, c_grp, min(c_grp + PD_JOIN - 1, c1), 1, c0);
+      __syncthreads();
+    }
+    if (finish && n_grps > 1) {
+      float* dst = p.part + place(c_grp) * NQ * PD_PART;
+      for (int col = warp; col < n_q; col += PD_WARPS) {
+        const Sums x = mine(col);
+        __stcg(reinterpret_cast<float4*>(dst + col * PD_PART) + lane, x.num);
+        if (lane == 0) __stcg(reinterpret_cast<float2*>(dst + col * PD_PART + 128), make_float2(x.ref, x.den));
       }
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
         int* tk = p.tickets + ((int64_t)b * HH + hh);
-        const int drawn = atomicAdd(tk, 1);
-        sm_last = drawn == (int)(c1 - c0);
-        if (sm_last) *tk = 0;                                        // every other one has been drawn
+        sm_last = atomicAdd(tk, 1) == n_grps - 1;
+        if (sm_last) *tk = 0;
       }
       __syncthreads();
       finish = sm_last != 0;
-      if (finish) __threadfence();
+      if (finish) {
+        __threadfence();
+        join_shares<NQ>(p.part, &sm_acc[0][0][0], &sm_m[0][0], &sm_l[0][0], n_q, c0, c1, PD_JOIN, c0);
+        __syncthreads();
+      }
     }
     if (finish) {
-      // ---------------------------------------------------------------- the token's own row
-      if (r.len >= 0) {
-        float kr[4], vr[4];
-        row_of_warp(p.k + b * p.k_sb + h * p.k_sh, p.flags & DAISY_NORM_K, p.flags & DAISY_ROPE, p.eps, cos_row, sin_row, lane, kr);
-        row_of_warp(p.v + b * p.v_sb + h * p.v_sh, p.flags & DAISY_NORM_V, false, p.eps, cos_row, sin_row, lane, vr);
-        if (p.ve) {
-          const float gate = 1.0f / (1.0f + __expf(-*p.ve_gate));
-          const uint2 u = *reinterpret_cast<const uint2*>(p.ve + b * p.ve_sb + h * p.ve_sh + 4 * lane);
-          const float e[4] = {bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y)};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) vr[i] = gate * vr[i] + (1.0f - gate) * e[i];
-        }
-        const uint2 k16 = make_uint2(pack16<F16>(kr[0], kr[1]), pack16<F16>(kr[2], kr[3]));
-        const uint2 v16 = make_uint2(pack16<F16>(vr[0], vr[1]), pack16<F16>(vr[2], vr[3]));
-        const float2 ka = unpack16<F16>(k16.x), kc = unpack16<F16>(k16.y), va = unpack16<F16>(v16.x), vc = unpack16<F16>(v16.y);
-        for (int col = warp; col < n_q; col += PD_WARPS) {
-          float x[4];
-          row_of_warp(p.q + b * p.q_sb + (q_h0 + col) * p.q_sh, p.flags & DAISY_NORM_Q, p.flags & DAISY_ROPE, p.eps, cos_row, sin_row, lane, x);
-          const float s = warp_sum(x[0] * ka.x + x[1] * ka.y + x[2] * kc.x + x[3] * kc.y) * p.qscale;
-          if (lane == 0) sm_self[col] = s;
-        }
-        if (warp == 0) {
-          *reinterpret_cast<float4*>(&sm_v[4 * lane]) = make_float4(va.x, va.y, vc.x, vc.y);
-          if (grp == 0) {
-            const int new_pg = __ldcg(table + (r.len >> p.c.lg));
-            if ((unsigned)new_pg < (unsigned)p.c.n_pages) {
-              const int64_t at = p.c.at(new_pg, h, r.len) + 8 * lane;
-              *reinterpret_cast<uint2*>(p.c.k + at) = k16;
-              *reinterpret_cast<uint2*>(p.c.v + at) = v16;
-            } else if (p.status && lane == 0) {
-              p.status[0] = DAISY_EINVAL;
-            }
-          }
+      if (warp == PD_WARPS - 1 && grp == 0 && r.len >= 0) {
+        if ((unsigned)sm_own.page < (unsigned)p.c.n_pages) {
+          const int64_t at = p.c.at(sm_own.page, h, r.len) + 8 * lane;
+          *reinterpret_cast<uint2*>(p.c.k + at) = sm_own.k16[lane];
+          *reinterpret_cast<uint2*>(p.c.v + at) = sm_own.v16[lane];
+        } else if (p.status && lane == 0) {
+          p.status[0] = DAISY_EINVAL;
         }
       }
-      __syncthreads();
-      for (int col = 0; col < n_q; ++col) {
-        float y = 0.f;
+      for (int col = warp; col < n_q; col += PD_WARPS) {
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
         if (r.len >= 0) {
-          float num, ref, den;
-          if (alone) {
-            mine(col, num, ref, den);
-          } else {
-            ref = PD_NEG; num = den = 0.f;
-            for (int64_t cc = c0; cc <= c1; ++cc) {
-              const float* src = p.part + (cc * 2 + (cc == c0 ? 1 : 0)) * NQ * PD_PART + col * PD_PART;
-              const float n1 = __ldcg(src + d), r1 = __ldcg(src + 128), d1 = __ldcg(src + 129);
-              const float top = fmaxf(ref, r1), a = fast_exp2(ref - top), e = fast_exp2(r1 - top);
-              num = num * a + n1 * e;
-              den = den * a + d1 * e;
-              ref = top;
-            }
-          }
-          const float self = sm_self[col], top = fmaxf(ref, self), a = fast_exp2(ref - top), w = fast_exp2(self - top);
-          y = (num * a + w * sm_v[d]) / (den * a + w);
+          const Sums x = mine(col);
+          const float self = sm_self[col], top = fmaxf(x.ref, self), a = fast_exp2(x.ref - top), w = fast_exp2(self - top);
+          const float4 v = sm_own.v[lane];
+          const float inv = 1.0f / (x.den * a + w), ai = a * inv, wi = w * inv;
+          y = make_float4(x.num.x * ai + wi * v.x, x.num.y * ai + wi * v.y, x.num.z * ai + wi * v.z, x.num.w * ai + wi * v.w);
         }
-        p.out[b * p.o_sb + (q_h0 + col) * p.o_sh + d] = __float2bfloat16_rn(y);
+        __nv_bfloat16* dst = p.out + b * p.o_sb + (q_h0 + col) * p.o_sh + 4 * lane;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
       }
     }
     t = s_end;
@@ -452,13 +615,14 @@ static size_t partials_bytes(int sms) {
   constexpr size_t cols = pd_ctas(8) * 8 > pd_ctas(16) * 16 ? pd_ctas(8) * 8 : pd_ctas(16) * 16;
   return (size_t)sms * 2 * cols * PD_PART * sizeof(float);
 }
+static size_t group_tickets_bytes(int sms) { return (size_t)sms * 2 * pd_ctas(8) * sizeof(int); }
 
 extern "C" size_t daisy_b200_paged_decode_workspace_bytes(int n_seq, int Hq, int H, int D) {
   if (n_seq <= 0 || Hq <= 0 || H <= 0 || D != DAISY_HEAD_DIM || Hq % H) return 0;
   int sms = daisy_host::sm_count_cached();
   if (sms <= 0) sms = daisy_host::MAX_SMS;
   const int nq = decode_cols(Hq / H), n_grp = (Hq / H + nq - 1) / nq;
-  return partials_bytes(sms) + ((size_t)n_seq * H * n_grp * sizeof(int) + 15) / 16 * 16;
+  return partials_bytes(sms) + group_tickets_bytes(sms) + ((size_t)n_seq * H * n_grp * sizeof(int) + 15) / 16 * 16;
 }
 
 extern "C" int daisy_b200_paged_decode_step(const daisy_b200_pages* cache, const void* q_new, const void* k_new, const void* v_new,
@@ -476,7 +640,7 @@ extern "C" int daisy_b200_paged_decode_step(const daisy_b200_pages* cache, const
   if (ve && (!ve_gate_logit || !(flags & DAISY_NORM_V))) return DAISY_EINVAL;
   if (!daisy_aligned16(q_new) || !daisy_aligned16(k_new) || !daisy_aligned16(v_new) || !daisy_aligned16(ve) || !daisy_aligned16(workspace) ||
       ((q_sb | q_sh | k_sb | k_sh | v_sb | v_sh) & 7) || (ve && ((ve_sb | ve_sh) & 7)) || (reinterpret_cast<uintptr_t>(lens) & 3) ||
-      (reinterpret_cast<uintptr_t>(out) & 1))
+      (reinterpret_cast<uintptr_t>(out) & 7) || ((o_sb | o_sh) & 3))
     return DAISY_EALIGN;
   if ((flags & DAISY_ROPE) && (!daisy_aligned16(cos) || !daisy_aligned16(sin))) return DAISY_EALIGN;
   if (workspace_bytes < daisy_b200_paged_decode_workspace_bytes(cache->n_seq, Hq, cache->H, D)) return DAISY_EWORKSPACE;
@@ -485,7 +649,9 @@ extern "C" int daisy_b200_paged_decode_step(const daisy_b200_pages* cache, const
   p.G = Hq / cache->H; p.Hq = Hq;
   const int nq = decode_cols(p.G);
   p.n_grp = (p.G + nq - 1) / nq;
-  if ((int64_t)cache->n_seq * cache->H * p.n_grp >= (int64_t)1 << 31) return DAISY_EUNSUPPORTED;
+  // blocks are counted in 32 bits
+  const int64_t blocks = (int64_t)cache->width * cache->page / (PD_TILE * PD_WARPS) + 2 + PD_HEAD, pairs = (int64_t)cache->n_seq * cache->H * p.n_grp;
+  if (pairs >= (int64_t)1 << 31 || blocks * pairs >= ((int64_t)1 << 31) - 65536) return DAISY_EUNSUPPORTED;
   p.q = (const __nv_bfloat16*)q_new; p.k = (const __nv_bfloat16*)k_new; p.v = (const __nv_bfloat16*)v_new; p.ve = (const __nv_bfloat16*)ve;
   p.q_sb = q_sb; p.q_sh = q_sh; p.k_sb = k_sb; p.k_sh = k_sh; p.v_sb = v_sb; p.v_sh = v_sh; p.ve_sb = ve_sb; p.ve_sh = ve_sh;
   p.o_sb = o_sb; p.o_sh = o_sh;
@@ -496,7 +662,8 @@ extern "C" int daisy_b200_paged_decode_step(const daisy_b200_pages* cache, const
   p.eps = eps; p.flags = flags; p.status = status_word;
   const unsigned grid = (unsigned)(sms * pd_ctas(nq));
   p.part = (float*)workspace;
-  p.tickets = (int*)((char*)workspace + partials_bytes(sms));
+  p.tickets_grp = (int*)((char*)workspace + partials_bytes(sms));
+  p.tickets = (int*)((char*)p.tickets_grp + group_tickets_bytes(sms));
   const bool f16 = (flags & DAISY_CACHE_FP16) != 0;
   cudaStream_t st = (cudaStream_t)stream;
   auto go = [&](auto kernel) { return daisy_host::launch_dependent(kernel, dim3(grid), dim3(32 * PD_WARPS), 0, st, p); };
