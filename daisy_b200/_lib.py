@@ -93,9 +93,8 @@ SIGNATURES = {
     "daisy_b200_paged_decode_workspace_bytes": (_sz, [_i] * 4),
     "daisy_b200_paged_decode_step": (_i, [_vp] * 4 + [_i64] * 6 + [_vp, _i, _vp, _vp, _i] + [_vp, _i64, _i64] + [_vp, _i64, _i64, _vp] +
                                      [_i] * 2 + [_f, _f, _u, _vp, _sz, _vp, _vp]),
-    "daisy_b200_paged_attend_workspace_bytes": (_sz, [_i] * 4),
-    "daisy_b200_paged_attend_ticket_bytes": (_sz, []),
-    "daisy_b200_paged_attend": (_i, [_vp] * 2 + [_i64] * 3 + [_vp] * 2 + [_i, _vp] + [_i64] * 3 + [_i] * 4 + [_f, _u, _vp, _sz] + [_vp] * 3),
+    "daisy_b200_paged_attend_workspace_bytes": (_sz, [_i] * 5),
+    "daisy_b200_paged_attend": (_i, [_vp] * 2 + [_i64] * 3 + [_vp] * 2 + [_i, _vp] + [_i64] * 3 + [_i] * 4 + [_f, _u, _vp, _sz] + [_vp] * 2),
 }
 
 

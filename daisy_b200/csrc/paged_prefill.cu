@@ -1,10 +1,12 @@
 // Causal attention of a chunk of every sequence over a paged cache, on tcgen05 tensor cores.
 //
 // Query i of sequence b stands at position lens[b] - n_b + i and sees the nearest `window` keys up to its own, all of them in
-// the pages.  A work item is 256 queries (two 128-row streams that share every K/V tile; 128 where few) of one head; tiles of 128 keys.
-// Long items of a call with few of them are cut along the keys into pieces, whose sums (fp32) the last one to finish joins in
-// a fixed order.  The lengths are on the device, so a first, one-block launch works out the pieces, longest first, and the
-// attention kernel's CTAs draw them one by one.
+// the pages.  A work item is 256 rows (two 128-row streams that share every K/V tile; 128 where few) of `pack` query heads that
+// share a key head: row r is query r / pack, head r % pack, so that a few queries of grouped heads fill the rows.  Tiles of 128 keys.
+// Long items of a call with few of them are cut along the keys into pieces, whose sums (fp32) a last launch joins in their
+// order.  The lengths are on the device, so a first, one-block launch works out the pieces, longest first, and the attention
+// kernel's CTAs draw them one by one.  Where all sequences have as many queries and nothing would be cut, the items are counted off
+// instead, in one launch.
 //
 // Roles (as in the dense prefill kernel): two softmax warpgroups a stream, 64 key columns each, where the caller bounds the
 // logits (no running maximum is needed then), else one a stream with the whole row and a lazily refreshed reference maximum; a
@@ -15,6 +17,7 @@
 // scores are replaced, and the issuer clears their V rows in shared memory, since 0 x NaN is NaN in a product.
 // All waits are bounded, as in the dense kernel.
 #include "paged.cuh"
+#include <algorithm>
 
 namespace daisy {
 
@@ -26,24 +29,28 @@ constexpr int PP_SMEM = 1024 + PP_SMEM_TILES + PP_BARS;
 static_assert(PP_SMEM <= 232448, "over the 227 KB a CTA may use");
 constexpr float PP_NEG = -1.0e30f;
 
-// A piece: key tiles j0 .. j1 of the 256 (or 128) queries i0 .. of sequence b.  parts > 1: one of several, at slot + head * parts + part.
-struct __align__(32) Piece { int b, i0, j0, j1, slot, part, parts, pad; };
+// A piece: key tiles j0 .. j1 of the item of n queries i0 .. of sequence b, the first at position pos (negative: they see nothing), row row0 of q.
+// parts > 1: one of several, at slot + head * parts + part.
+struct __align__(16) Piece { int b, i0, j0, j1, slot, part, parts, pos, n, row0, pad[2]; };
 
-struct PlanHead { int n_pieces, queue, pad[6]; };
+struct Cut { int b, i0, slot, parts; };                              // an item in pieces, as Piece has them
+struct PlanHead { int n_pieces, queue, n_cuts, pad[5]; };
 
 struct PagedPrefillParams {
   PagedCache c;
   __nv_bfloat16* out;
   int64_t o_sb, o_st, o_sh;
   const int *lens, *cu;
-  int T, Hq, G, window, rows;        // rows: queries of an item
+  int T, Hq, G, window, toks;        // toks: queries of an item, 256 or 128 rows / pack
+  int lgp, heads;                    // pack = 1 << lgp; heads = Hq / pack
+  int counted;                       // > 0: items without a plan, so many a sequence
   float scale_log2;
   int* status;
   PlanHead* head;
   Piece* pieces;
+  Cut* cuts;
   float* part;                       // [slots][PP_SLOT]
-  int* tickets;                      // [slots][16], zero between calls
-  int slots, max_pieces;
+  int slots, max_pieces;             // slots = 0: nothing is cut
 };
 // a warp's share of a piece's sums: [columns][32 rows], then reference and denominator of the 32 rows
 constexpr int PP_SLOT = 2 * 8 * (64 * 32 + 64);                     // floats: 8 warps a stream x 64 columns (or 4 x 128)
@@ -73,116 +80,133 @@ __device__ __forceinline__ int last_tile(int pos, int n) { return (pos + n - 1) 
 
 // The pieces of a call, longest first.  One block; a warp a sequence, a lane an item.
 // How far items are cut: into pieces of at most L tiles, L from a few candidates by the estimate
-// total / CTAs + half a longest piece (+ four tiles' time for every piece of a cut item), or a longest piece where all pieces find a CTA.
-constexpr int PLAN_THREADS = 1024, PLAN_CAND = 6, PLAN_BUCKETS = 1024;
+// total / CTAs + half a longest piece, or a longest piece where all pieces find a CTA, and ten tiles' time for every piece of a cut item
+// (its sums are written, and read again by the last: 8192 tokens x 16 heads cut in halves 322 us, whole 278).
+constexpr float PLAN_COST = 8.f;
+constexpr int PLAN_THREADS = 1024, PLAN_CAND = 6, PLAN_BUCKETS = 1024, PLAN_KEPT = 1024;
+struct PlanItem { int b, i0, j0, j1, pos, n, row0; };               // j1 < j0: queries that see nothing
 __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PagedPrefillParams p, int ctas) {
+  __shared__ PlanItem kept[PLAN_KEPT];
   __shared__ int hist[PLAN_BUCKETS];
   __shared__ unsigned long long sm_total;
-  __shared__ int sm_longest, sm_items, sm_slots, sm_cut, sm_pieces[PLAN_CAND], sm_parts[PLAN_CAND], sm_L[PLAN_CAND];
+  __shared__ int sm_longest, sm_items, sm_slots, sm_cuts, sm_cut, sm_pieces[PLAN_CAND], sm_parts[PLAN_CAND], sm_L[PLAN_CAND], warp_sums[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < PLAN_BUCKETS; i += PLAN_THREADS) hist[i] = 0;
-  if (threadIdx.x == 0) { sm_total = 0; sm_longest = 0; sm_items = 0; sm_slots = 0; }
+  hist[threadIdx.x] = 0;
+  if (threadIdx.x == 0) { sm_total = 0; sm_longest = 0; sm_items = 0; sm_slots = 0; sm_cuts = 0; }
   if (threadIdx.x < PLAN_CAND) { sm_pieces[threadIdx.x] = 0; sm_parts[threadIdx.x] = 0; }
   grid_dep_launch();
   grid_dep_wait();
   __syncthreads();
-  // f(b, i0, j0, j1) for every item; j1 < j0: rows that see nothing
-  auto items = [&](auto f) {
+  // every item, from the lengths: a warp a sequence, a lane an item
+  auto count_off = [&](auto f) {
     for (int b = warp; b < p.c.n_seq; b += PLAN_THREADS / 32) {
       const SeqQueries s = seq_queries(p, b);
       if (s.refused && p.status && lane == 0) p.status[0] = DAISY_EINVAL;
-      for (int i0 = lane * p.rows; i0 < s.n; i0 += 32 * p.rows) {
-        if (s.pos < 0) f(b, i0, 1, 0);
-        else f(b, i0, first_tile(s.pos + i0, p.window), last_tile(s.pos + i0, min(p.rows, s.n - i0)));
+      for (int i0 = lane * p.toks; i0 < s.n; i0 += 32 * p.toks) {
+        PlanItem it{b, i0, 1, 0, -1, min(p.toks, s.n - i0), s.row0 + i0};
+        if (s.pos >= 0) { it.pos = s.pos + i0; it.j0 = first_tile(it.pos, p.window); it.j1 = last_tile(it.pos, it.n); }
+        f(it);
       }
     }
   };
   {
-    unsigned long long total = 0;
-    int longest = 0, n = 0;
-    items([&](int, int, int j0, int j1) { const int t = j1 - j0 + 1; total += t; longest = max(longest, t); ++n; });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      total += __shfl_xor_sync(0xffffffffu, total, o);
-      longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-      n += __shfl_xor_sync(0xffffffffu, n, o);
-    }
-    if (lane == 0 && n > 0) { atomicAdd(&sm_total, total); atomicMax(&sm_longest, longest); atomicAdd(&sm_items, n); }
+    unsigned total = 0;
+    int longest = 0;
+    count_off([&](const PlanItem& it) {
+      const int at = atomicAdd(&sm_items, 1), t = it.j1 - it.j0 + 1;
+      if (at < PLAN_KEPT) kept[at] = it;
+      total += t;
+      longest = max(longest, t);
+    });
+    total = __reduce_add_sync(0xffffffffu, total);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 0 && longest > 0) { atomicAdd(&sm_total, (unsigned long long)total); atomicMax(&sm_longest, longest); }
   }
   __syncthreads();
+  const int n_items = sm_items;
+  auto items = [&](auto f) {                                         // again: a thread an item where they were kept
+    if (n_items <= PLAN_KEPT) { if ((int)threadIdx.x < n_items) f(kept[threadIdx.x]); }
+    else count_off(f);
+  };
   if (threadIdx.x < PLAN_CAND) {
-    const int fit = sm_items > 0 ? ctas / max(1, sm_items * p.Hq) : 1;
+    const int fit = n_items > 0 ? ctas / max(1, n_items * p.heads) : 1;
     const int n = threadIdx.x == 0 ? 1 : threadIdx.x == 1 ? max(1, fit) : threadIdx.x;             // whole; as many as find a CTA; 2, 3, 4, 5
     sm_L[threadIdx.x] = max((sm_longest + n - 1) / n, min(4, max(sm_longest, 1)));
   }
-  __syncthreads();
-  {
+  if (p.slots > 0) {
+    __syncthreads();
     int pieces[PLAN_CAND] = {}, parts[PLAN_CAND] = {};
-    items([&](int, int, int j0, int j1) {
-      const int t = max(j1 - j0 + 1, 1);
+    items([&](const PlanItem& it) {
+      const unsigned t = max(it.j1 - it.j0 + 1, 1);
 #pragma unroll
       for (int k = 0; k < PLAN_CAND; ++k) {
-        const int n = (t + sm_L[k] - 1) / sm_L[k];
+        const int n = (int)((t + sm_L[k] - 1) / (unsigned)sm_L[k]);
         pieces[k] += n;
         if (n > 1) parts[k] += n;
       }
     });
 #pragma unroll
     for (int k = 0; k < PLAN_CAND; ++k) {
-      if (pieces[k]) atomicAdd(&sm_pieces[k], pieces[k]);
-      if (parts[k]) atomicAdd(&sm_parts[k], parts[k]);
+      const int a = __reduce_add_sync(0xffffffffu, pieces[k]), e = __reduce_add_sync(0xffffffffu, parts[k]);
+      if (lane == 0 && a) { atomicAdd(&sm_pieces[k], a); atomicAdd(&sm_parts[k], e); }
     }
   }
   __syncthreads();
   if (threadIdx.x == 0) {
     float best = 3.0e38f;
-    int cut = 0;
-    for (int k = 0; k < PLAN_CAND; ++k) {
-      const int64_t n = (int64_t)sm_pieces[k] * p.Hq, parts = (int64_t)sm_parts[k] * p.Hq;
+    int cut = sm_L[0];
+    for (int k = 0; k < PLAN_CAND && p.slots > 0; ++k) {
+      const int64_t n = (int64_t)sm_pieces[k] * p.heads, parts = (int64_t)sm_parts[k] * p.heads;
       if (k > 0 && (parts > p.slots || sm_pieces[k] > p.max_pieces)) continue;
-      const float share = (float)sm_total * p.Hq / ctas;
-      const float est = (n <= ctas ? (float)sm_L[k] : share + 0.5f * sm_L[k]) + (parts > 0 ? 4.f * fmaxf(1.f, (float)parts / ctas) : 0.f);
+      const float share = (float)sm_total * p.heads / ctas;
+      const float est = (n <= ctas ? (float)sm_L[k] : share + 0.5f * sm_L[k]) + (parts > 0 ? PLAN_COST * fmaxf(1.f, (float)parts / ctas) : 0.f);
       if (est < best) { best = est; cut = sm_L[k]; }
     }
-    sm_cut = cut;
+    sm_cut = max(cut, 1);
   }
   __syncthreads();
-  const int L = max(sm_cut, 1);
-  auto bucket = [](int t) { return PLAN_BUCKETS - 1 - min(max(t, 0), PLAN_BUCKETS - 1); };          // longest first
-  auto pieces_of = [&](int j0, int j1, auto f) {
-    const int t = j1 - j0 + 1, n = max(1, (t + L - 1) / L);
-    for (int i = 0; i < n; ++i) f(j0 + (int)((int64_t)t * i / n), n == 1 ? j1 : j0 + (int)((int64_t)t * (i + 1) / n) - 1, i, n);
-  };
-  items([&](int, int, int j0, int j1) { pieces_of(j0, j1, [&](int a, int e, int, int) { atomicAdd(&hist[bucket(e - a + 1)], 1); }); });
+  const unsigned L = sm_cut;
+  auto bucket = [](int t) { return PLAN_BUCKETS - 1 - min(t, PLAN_BUCKETS - 1); };                  // longest first
+  // an item of t tiles goes in n pieces: t % n of them one tile longer than the others
+  items([&](const PlanItem& it) {
+    const int t = it.j1 - it.j0 + 1, n = max(1, (int)((t + L - 1) / L)), rem = t % n;
+    if (rem) atomicAdd(&hist[bucket(t / n + 1)], rem);
+    atomicAdd(&hist[bucket(t / n)], n - rem);
+  });
   __syncthreads();
-  // exclusive prefix sums of the 1024 buckets
-  __shared__ int warp_sums[32];
-  {
+  {                                                                  // exclusive prefix sums of the buckets, a thread each
     const int own = hist[threadIdx.x];
     int x = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
-    int base = 0;
-    for (int w = 0; w < warp; ++w) base += warp_sums[w];
-    hist[threadIdx.x] = base + x - own;
-    if (threadIdx.x == PLAN_THREADS - 1) { p.head->n_pieces = min(base + x, p.max_pieces); p.head->queue = 0; }
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane] : 0);
+    hist[threadIdx.x] = before + x - own;
+    if (threadIdx.x == PLAN_THREADS - 1) { p.head->n_pieces = min(before + x, p.max_pieces); p.head->queue = 0; }
   }
   __syncthreads();
-  items([&](int b, int i0, int j0, int j1) {
-    const int n = max(1, (j1 - j0 + L) / L);
-    const int slot = n > 1 ? atomicAdd(&sm_slots, n * p.Hq) : 0;
-    pieces_of(j0, j1, [&](int a, int e, int i, int parts) {
-      const int at = atomicAdd(&hist[bucket(e - a + 1)], 1);
-      if (at < p.max_pieces) p.pieces[at] = Piece{b, i0, a, e, slot, i, parts, 0};
-    });
+  items([&](const PlanItem& it) {
+    const int t = it.j1 - it.j0 + 1, n = max(1, (int)((t + L - 1) / L)), rem = t % n, len = t / n;
+    int slot = 0;
+    if (n > 1) {
+      slot = atomicAdd(&sm_slots, n * p.heads);
+      p.cuts[atomicAdd(&sm_cuts, 1)] = Cut{it.b, it.i0, slot, n};
+    }
+    const int at_long = rem ? atomicAdd(&hist[bucket(len + 1)], rem) : 0, at_short = atomicAdd(&hist[bucket(len)], n - rem);
+    auto put = [&](int i) {
+      const int j = it.j0 + i * len + min(i, rem), at = i < rem ? at_long + i : at_short + i - rem;
+      if (at < p.max_pieces) p.pieces[at] = Piece{it.b, it.i0, j, j + len - (i < rem ? 0 : 1), slot, i, n, it.pos, it.n, it.row0, {0, 0}};
+    };
+    for (int i = 0; i < n; ++i) put(i);
   });
+  __syncthreads();
+  if (threadIdx.x == 0) p.head->n_cuts = sm_cuts;
 }
 
 struct PagedItem {
-  int b, h;                          // b < 0: no more
-  int q0[2], n[2], jlo_s[2], jhi_s[2];
+  int b, h;                          // b < 0: no more; h counts packs of heads
+  int q0[2], n[2], jlo_s[2], jhi_s[2];      // of each stream: first position, queries, key tiles
   bool valid[2];                     // has tiles in this piece
   int jlo, jhi;
   int see0, end;                     // keys see0 .. end - 1 are seen by some row of the item
@@ -254,7 +278,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   if (warp == TMA_WARP) {
     // ------------------------------------------------------------------ TMA producer: the warp as one, lane 0 issues
     if (lane == 0) { prefetch_tmap(&tm_q); prefetch_tmap(&tm_k); prefetch_tmap(&tm_v); }
-    const int n_work = __ldcg(&p.head->n_pieces) * p.Hq;            // L2: this grid was there before the plan was written
+    // the plan's words come from L2: this grid was there before they were written
+    int n_work = p.counted * p.c.n_seq * p.heads;                   // with a plan: known with the first piece
+    const int ts = PP_BM >> p.lgp;                                  // queries of a stream
     const int lgr = min(p.c.lg, 7), boxes = PP_BN >> lgr;           // a tile is `boxes` boxes of 1 << lgr rows
     int n = 0;
     uint32_t qn[2] = {0, 0};
@@ -271,13 +297,14 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         uint8_t* dst = q_tiles + (qb * 2 + s) * PP_TILE;
         if (lane == 0) {
           mbar_expect_tx(&bars->q_full[s][qb], PP_TILE);
-          tma_load_4d(dst, &tm_q, &bars->q_full[s][qb], 0, g.row0 + s * PP_BM, g.h, g.bq);
-          tma_load_4d(dst + PP_HALF, &tm_q, &bars->q_full[s][qb], 64, g.row0 + s * PP_BM, g.h, g.bq);
+          tma_load_4d(dst, &tm_q, &bars->q_full[s][qb], 0, g.h << p.lgp, g.row0 + s * ts, g.bq);
+          tma_load_4d(dst + PP_HALF, &tm_q, &bars->q_full[s][qb], 64, g.h << p.lgp, g.row0 + s * ts, g.bq);
         }
       }
     };
     int drawn = blockIdx.x;                                         // the first one is this CTA's own number, later ones are drawn
     auto draw = [&]() {
+      if (p.counted > 0) { drawn += gridDim.x; return; }
       int x = 0;
       if (lane == 0) x = atomicAdd(&p.head->queue, 1);
       drawn = (int)gridDim.x + __shfl_sync(0xffffffffu, x, 0);
@@ -285,24 +312,36 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     auto publish = [&](int rd, PagedItem& g) {
       const int slot = rd % PP_NITEM;
       g.b = -1;
-      if (drawn < n_work) {
-        const int at = drawn / p.Hq;
-        const int4* src = reinterpret_cast<const int4*>(p.pieces + at);
-        const int4 lo = __ldcg(src), hi = __ldcg(src + 1);
-        const Piece pc{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        const SeqQueries sq = seq_queries(p, pc.b);
-        g.b = pc.b; g.h = drawn - at * p.Hq;
+      Piece pc;
+      bool there = false;
+      if (p.counted > 0) {                                           // a sequence's last queries first: they see most
+        there = drawn < n_work;
+        if (there) {
+          const int at = drawn / p.heads, i = at / p.c.n_seq, i0 = (p.counted - 1 - i) * p.toks, b = at - i * p.c.n_seq;
+          const SeqQueries sq = seq_queries(p, b);
+          if (sq.refused && p.status && lane == 0) p.status[0] = DAISY_EINVAL;
+          pc = Piece{b, i0, 0, 1 << 30, 0, 0, 1, sq.pos < 0 ? -1 : sq.pos + i0, min(p.toks, sq.n - i0), sq.row0 + i0, {0, 0}};
+        }
+      } else if (drawn / p.heads < p.max_pieces) {
+        const int4* src = reinterpret_cast<const int4*>(p.pieces + drawn / p.heads);
+        const int4 x = __ldcg(src), y = __ldcg(src + 1), z = __ldcg(src + 2);
+        if (rd == 0) n_work = __ldcg(&p.head->n_pieces) * p.heads;
+        there = drawn < n_work;
+        pc = Piece{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w, z.x, z.y, {0, 0}};
+      }
+      if (there) {
+        g.b = pc.b; g.h = drawn % p.heads;
         g.bq = p.cu ? 0 : pc.b;
-        g.row0 = sq.row0 + pc.i0;
+        g.row0 = pc.row0;
         g.slot = pc.slot + g.h * pc.parts; g.part = pc.part; g.parts = pc.parts;
-        const int pos = sq.pos + pc.i0;
+        const int pos = pc.pos;
         g.jlo = 1 << 30; g.jhi = -1;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          g.q0[s] = pos + s * PP_BM;
-          g.n[s] = min(max(min(p.rows, sq.n - pc.i0) - s * PP_BM, 0), PP_BM);
+          g.q0[s] = pos + s * ts;
+          g.n[s] = min(max(pc.n - s * ts, 0), ts);
           g.jlo_s[s] = 1; g.jhi_s[s] = 0;
-          if (g.n[s] > 0 && sq.pos >= 0) {
+          if (g.n[s] > 0 && pos >= 0) {
             g.jlo_s[s] = max(first_tile(g.q0[s], p.window), pc.j0);
             g.jhi_s[s] = min(last_tile(g.q0[s], g.n[s]), pc.j1);
           }
@@ -325,7 +364,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     for (int rd = 0; ok && g.b >= 0; ++rd, g = g_next) {
       // the table's entries, a lane each, 32 at a time, the next 32 on their way
       const int* table = p.c.table + g.b * p.c.table_sb;
-      const int e_first = g.see0 >> p.c.lg, e_last = (g.end - 1) >> p.c.lg, hk = g.h / p.G;
+      const int e_first = g.see0 >> p.c.lg, e_last = (g.end - 1) >> p.c.lg, hk = (g.h << p.lgp) / p.G;
       auto entries = [&](int from) {
         const int i = from + lane;
         return i >= e_first && i <= e_last ? __ldcg(table + i) : 0;
@@ -455,7 +494,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     constexpr int COLS = 128 / NSPLIT;                               // of the scores, and of the output in the epilogue
     const int grp = warp >> 2, quarter = warp & 3;
     const int s = NSPLIT == 2 ? grp & 1 : grp, half = NSPLIT == 2 ? grp >> 1 : 0;
-    const int row = quarter * 32 + lane;
+    const int row = quarter * 32 + lane, ts = PP_BM >> p.lgp, pack1 = (1 << p.lgp) - 1;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_tmem = tmem_base + lane_off + s * 128 + half * 64;
     const uint32_t o_tmem = tmem_base + lane_off + 256 + s * 128 + half * 64;
@@ -464,51 +503,26 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     bool ok = true;
     const PagedItem* item;
 
+    auto row_at = [&](const PagedItem* g, int r) {                   // row r of this stream: query r / pack, head r % pack
+      return p.out + g->bq * p.o_sb + (int64_t)(g->row0 + s * ts + (r >> p.lgp)) * p.o_st + (int64_t)((g->h << p.lgp) + (r & pack1)) * p.o_sh;
+    };
     // rows of this warp to the output, straight from registers
     auto store_row = [&](const PagedItem* g, const float* y) {       // y: COLS values of this lane's row
-      if (row >= g->n[s]) return;
-      __nv_bfloat16* dst = p.out + g->bq * p.o_sb + (int64_t)(g->row0 + s * PP_BM + row) * p.o_st + g->h * p.o_sh + half * 64;
+      if (row >= g->n[s] << p.lgp) return;
+      __nv_bfloat16* dst = row_at(g, row) + half * 64;
 #pragma unroll
       for (int c = 0; c < COLS; c += 8) *reinterpret_cast<uint4*>(dst + c) = pack8(y + c);
     };
-    // this warp's share of a cut item: left in the slot; the last warp to come joins the pieces in their order
-    auto join = [&](const PagedItem* g, const uint32_t* o, float m, float l) {
-      constexpr int SHARE = COLS * 32 + 64;
-      auto share = [&](int part) { return p.part + (int64_t)(g->slot + part) * PP_SLOT + ((s * NSPLIT + half) * 4 + quarter) * SHARE; };
-      float* dst = share(g->part);
-      if (l > 0.f || !(l == l)) {
+    // this warp's sums of a piece, for the launch that joins them
+    auto leave = [&](const PagedItem* g, const uint32_t* o, float m, float l) {
+      if (row >= g->n[s] << p.lgp) return;
+      float* dst = p.part + (int64_t)(g->slot + g->part) * PP_SLOT + ((s * NSPLIT + half) * 4 + quarter) * (COLS * 32 + 64) + lane;
+      if (l != 0.f) {                                                // else the row sees none of the piece
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) dst[c * 32 + lane] = __uint_as_float(o[c]);
+        for (int c = 0; c < COLS; ++c) dst[c * 32] = __uint_as_float(o[c]);
       }
-      dst[COLS * 32 + lane] = m;
-      dst[COLS * 32 + 32 + lane] = l;
-      __threadfence();
-      __syncwarp();
-      int last = 0;
-      if (lane == 0) {
-        int* tk = p.tickets + (int64_t)g->slot * 16 + (s * NSPLIT + half) * 4 + quarter;
-        last = atomicAdd(tk, 1) == g->parts - 1;
-        if (last) *tk = 0;
-      }
-      if (!__shfl_sync(0xffffffffu, last, 0)) return;
-      __threadfence();
-      float y[COLS], M = PP_NEG, den = 0.f;
-#pragma unroll
-      for (int c = 0; c < COLS; ++c) y[c] = 0.f;
-      for (int i = 0; i < g->parts; ++i) {
-        const float* src = share(i);
-        const float m1 = __ldcg(src + COLS * 32 + lane), l1 = __ldcg(src + COLS * 32 + 32 + lane);
-        if (l1 == 0.f) continue;                                     // this lane's row sees none of that piece
-        const float top = fmaxf(M, m1), a = fast_exp2(M - top), e = fast_exp2(m1 - top);
-        den = den * a + l1 * e;
-        M = top;
-#pragma unroll
-        for (int c = 0; c < COLS; ++c) y[c] = y[c] * a + __ldcg(src + c * 32 + lane) * e;
-      }
-      const float inv = 1.0f / den;
-#pragma unroll
-      for (int c = 0; c < COLS; ++c) y[c] *= inv;
-      store_row(g, y);
+      dst[COLS * 32] = m;
+      dst[COLS * 32 + 32] = l;
     };
     // rows of an item that this warp's stream has no tiles of
     auto without_tiles = [&](const PagedItem* g) {
@@ -517,7 +531,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       float none[COLS];
 #pragma unroll
       for (int c = 0; c < COLS; ++c) { zero[c] = 0; none[c] = 0.f; }
-      if (g->parts > 1) join(g, zero, PP_NEG, 0.f);
+      if (g->parts > 1) leave(g, zero, PP_NEG, 0.f);
       else store_row(g, none);
     };
     // the last step of an item: l, m of this lane's row, sums in O.  box: 32 rows of 128 bytes (two with NSPLIT = 1) of the item's Q buffer,
@@ -528,11 +542,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       for (int c = 0; c < COLS; c += 32) tmem_ld32(o_tmem + c, o + c);
       tc_wait_ld();
       if (g->parts > 1) {
-        join(g, o, m, l);
+        leave(g, o, m, l);
       } else {
         const float inv = 1.0f / l;
-        __nv_bfloat16* dst = p.out + g->bq * p.o_sb + (int64_t)(g->row0 + s * PP_BM + quarter * 32) * p.o_st + g->h * p.o_sh + half * 64 + (lane & 7) * 8;
-        const int n_rows = g->n[s] - quarter * 32;
+        const int n_rows = (g->n[s] << p.lgp) - quarter * 32;
 #pragma unroll
         for (int hc = 0; hc < COLS / 64; ++hc) {
           uint8_t* mine = box + hc * PP_HALF;
@@ -548,7 +561,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           for (int i = 0; i < 8; ++i) {
             const int r = i * 4 + (lane >> 3);
             const uint4 v = *reinterpret_cast<const uint4*>(mine + (quarter * 32 + r) * 128 + (((lane & 7) ^ (r & 7)) << 4));
-            if (r < n_rows) *reinterpret_cast<uint4*>(dst + (int64_t)r * p.o_st + hc * 64) = v;
+            if (r < n_rows) *reinterpret_cast<uint4*>(row_at(g, quarter * 32 + r) + half * 64 + (lane & 7) * 8 + hc * 64) = v;
           }
         }
       }
@@ -563,7 +576,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     for (int rd = 0; ok && (item = next_item(rd)); item_done(rd), ++rd) {
       const int q0 = item->q0[s], jlo = item->jlo_s[s], jhi = item->jhi_s[s];
       if (jhi < jlo) { without_tiles(item); continue; }
-      const int q_row = q0 + row;
+      const int q_row = q0 + (row >> p.lgp);
       uint8_t* q_buf = q_tiles + ((n_o % PP_NQBUF) * 2 + s) * PP_TILE;
       auto scores_there = [&]() -> bool {
         const bool there = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[s], n_s & 1, abort_flag, p.status, 6));
@@ -577,7 +590,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         mbar_arrive(&bars->p_full[s]);
       };
       // whole tiles: all rows of the stream see all of their keys
-      const int f_lo = p.window > 0 ? max(q0 + PP_BM + PP_BN - 1 - p.window, 0) / PP_BN : 0, f_hi = (q0 + 1) / PP_BN - 1;
+      const int f_lo = p.window > 0 ? max(q0 + ts + PP_BN - 1 - p.window, 0) / PP_BN : 0, f_hi = (q0 + 1) / PP_BN - 1;
       if constexpr (NSPLIT == 2) {
         const uint64_t c2p = pack2f(c2, c2);
         uint64_t sum_a = pack2f(0.f, 0.f), sum_b = sum_a;
@@ -753,9 +766,76 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   }
 }
 
+// The pieces of cut items joined in their order.  A warp takes 32 rows and 16 of their columns, a lane a row, four pieces' sums in flight.
+template <int NSPLIT>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedPrefillParams p) {
+  constexpr int COLS = 128 / NSPLIT, SHARE = COLS * 32 + 64, CHUNK = 16;
+  const int lane = threadIdx.x & 31;
+  grid_dep_launch();
+  grid_dep_wait();
+  const int ts = PP_BM >> p.lgp;
+  const int64_t n_work = (int64_t)__ldcg(&p.head->n_cuts) * p.heads * (8 * NSPLIT) * (COLS / CHUNK);
+  for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < n_work; w += (int64_t)gridDim.x * 8) {
+    const int chunk = (int)(w % (COLS / CHUNK)), place = (int)(w / (COLS / CHUNK) % (8 * NSPLIT));
+    const int64_t item = w / (COLS / CHUNK) / (8 * NSPLIT);
+    const int h = (int)(item % p.heads);
+    const int4 c4 = __ldcg(reinterpret_cast<const int4*>(p.cuts + item / p.heads));
+    const Cut cut{c4.x, c4.y, c4.z, c4.w};
+    const int s = place / (4 * NSPLIT), half = place / 4 % NSPLIT, quarter = place % 4, row = quarter * 32 + lane;
+    const SeqQueries sq = seq_queries(p, cut.b);
+    const int rows = min(max(min(p.toks, sq.n - cut.i0) - s * ts, 0), ts) << p.lgp;
+    if (row >= rows) continue;
+    const float* base = p.part + (int64_t)(cut.slot + h * cut.parts) * PP_SLOT + place * SHARE + lane;
+    float M = PP_NEG, den = 0.f, y[CHUNK];
+#pragma unroll
+    for (int c = 0; c < CHUNK; ++c) y[c] = 0.f;
+    if (NSPLIT == 1)                                                 // with bounded logits all references are zero
+      for (int i = 0; i < cut.parts; ++i)
+        if (__ldcg(base + (int64_t)i * PP_SLOT + COLS * 32 + 32) != 0.f) M = fmaxf(M, __ldcg(base + (int64_t)i * PP_SLOT + COLS * 32));
+    for (int i0 = 0; i0 < cut.parts; i0 += 4) {
+      float x[4][CHUNK], l[4], m[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float* src = base + (int64_t)min(i0 + k, cut.parts - 1) * PP_SLOT;
+#pragma unroll
+        for (int c = 0; c < CHUNK; ++c) x[k][c] = __ldcg(src + (chunk * CHUNK + c) * 32);
+        m[k] = __ldcg(src + COLS * 32);
+        l[k] = __ldcg(src + COLS * 32 + 32);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i0 + k < cut.parts && l[k] != 0.f) {
+          const float e = NSPLIT == 1 ? fast_exp2(m[k] - M) : 1.f;
+          den = fmaf(l[k], e, den);
+#pragma unroll
+          for (int c = 0; c < CHUNK; ++c) y[c] = fmaf(x[k][c], e, y[c]);
+        }
+    }
+    const float inv = 1.0f / den;
+#pragma unroll
+    for (int c = 0; c < CHUNK; ++c) y[c] *= inv;
+    const int bq = p.cu ? 0 : cut.b, tok = sq.row0 + cut.i0 + s * ts + (row >> p.lgp), head = (h << p.lgp) + (row & ((1 << p.lgp) - 1));
+    __nv_bfloat16* dst = p.out + bq * p.o_sb + (int64_t)tok * p.o_st + (int64_t)head * p.o_sh + half * 64 + chunk * CHUNK;
+    *reinterpret_cast<uint4*>(dst) = pack8(y);
+    *reinterpret_cast<uint4*>(dst + 8) = pack8(y + 8);
+  }
+}
+
 }  // namespace daisy
 
 using namespace daisy;
+
+// Queries [B,T,H,D] as (d, h, t, b) with byte strides: a box of `heads` heads and `queries` queries is 128 rows of 64 channels, heads fastest;
+// 128-byte swizzle, zero fill out of bounds.
+static int make_tmap_packed_rows(CUtensorMap* m, const void* base, uint64_t D, uint64_t H, uint64_t T, uint64_t B, uint64_t sh, uint64_t st, uint64_t sb,
+                                 uint32_t heads, uint32_t queries) {
+  daisy_host::EncodeTiledFn enc = daisy_host::get_encode_tiled();
+  if (!enc) return DAISY_ECUDA;
+  cuuint64_t dims[4] = {D, H, T, B}, strides[3] = {sh, st, sb};
+  cuuint32_t box[4] = {64, heads, queries, 1}, estr[4] = {1, 1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? DAISY_OK : DAISY_ECUDA;
+}
 
 static int paged_prefill_smem() {
   static bool done[daisy_host::MAX_DEVICES] = {};             // the attribute is per device
@@ -770,54 +850,67 @@ static int paged_prefill_smem() {
 
 // Workspace: the plan's head, pieces and sums.
 constexpr int PP_SLOTS_PER_SM = 4;
-struct PrefillRoom { int slots; int64_t max_pieces; size_t head, pieces, part, end; };
-static PrefillRoom prefill_room(int sms, int64_t tokens, int n_seq, int rows) {
+struct PrefillRoom { int slots; int64_t max_pieces; size_t pieces, cuts, part, end; };
+static PrefillRoom prefill_room(int sms, int64_t tokens, int n_seq, int toks) {
   PrefillRoom r;
   r.slots = sms * PP_SLOTS_PER_SM;
   // items, and the further pieces of those that are cut
-  r.max_pieces = tokens / rows + n_seq + r.slots;
-  r.head = 0;
-  r.pieces = r.head + 256;
-  r.part = r.pieces + ((size_t)r.max_pieces * sizeof(Piece) + 255) / 256 * 256;
+  r.max_pieces = tokens / toks + n_seq + r.slots;
+  r.pieces = 256;
+  r.cuts = r.pieces + ((size_t)r.max_pieces * sizeof(Piece) + 255) / 256 * 256;
+  r.part = r.cuts + ((size_t)r.slots * sizeof(Cut) + 255) / 256 * 256;
   r.end = r.part + (size_t)r.slots * PP_SLOT * sizeof(float);
   return r;
 }
-// 128 queries an item where all items of that size find an SM: two streams pay by sharing K and V, not for latency
-static int prefill_rows(int sms, int64_t tokens, int n_seq, int Hq) { return (tokens / PP_BM + n_seq) * Hq <= sms ? PP_BM : 2 * PP_BM; }
-
-extern "C" size_t daisy_b200_paged_attend_ticket_bytes(void) {
-  int sms = daisy_host::sm_count_cached();
-  if (sms <= 0) sms = daisy_host::MAX_SMS;
-  return (size_t)sms * PP_SLOTS_PER_SM * 16 * sizeof(int);
+// query heads of a key head that lie in one item's rows: the largest power of two, 16 at most, that divides the group
+static int prefill_lgp(int G) {
+  int l = 0;
+  while (l < 4 && G % (2 << l) == 0) ++l;
+  return l;
+}
+// Queries of an item: 256 rows, or 128 where all items of that size find an SM and no item is long (`longest`: key tiles that the table or
+// the window leaves).  A tile takes one stream as long as two (1.57 us), so that the second one costs only where it adds tiles: 128 queries of
+// 8 heads over one key head and 131000 keys 102 us with items of 128 rows, 69 with 256.
+constexpr int64_t PP_SHORT = 16;
+static int prefill_toks(int sms, int64_t tokens, int n_seq, int Hq, int lgp, int64_t longest) {
+  const int solo = PP_BM >> lgp;
+  return longest <= PP_SHORT && (tokens / solo + n_seq) * (Hq >> lgp) <= sms ? solo : 2 * solo;
 }
 
-extern "C" size_t daisy_b200_paged_attend_workspace_bytes(int B, int T, int n_seq, int Hq) {
-  if (B <= 0 || T <= 0 || n_seq <= 0 || Hq <= 0) return 0;
+extern "C" size_t daisy_b200_paged_attend_workspace_bytes(int B, int T, int n_seq, int Hq, int H) {
+  if (B <= 0 || T <= 0 || n_seq <= 0 || Hq <= 0 || H <= 0 || Hq % H) return 0;
   int sms = daisy_host::sm_count_cached();
   if (sms <= 0) sms = daisy_host::MAX_SMS;
-  return prefill_room(sms, (int64_t)B * T, n_seq, prefill_rows(sms, (int64_t)B * T, n_seq, Hq)).end;
+  const int lgp = prefill_lgp(Hq / H);
+  return prefill_room(sms, (int64_t)B * T, n_seq, PP_BM >> lgp).end;                       // room for the smaller items
 }
 
 extern "C" int daisy_b200_paged_attend(const daisy_b200_pages* cache, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
                                        const int32_t* lens, const int32_t* cu, int window,
                                        void* out, int64_t o_sb, int64_t o_st, int64_t o_sh,
                                        int B, int T, int Hq, int D, float scale, unsigned flags,
-                                       void* workspace, size_t workspace_bytes, int32_t* tickets, int* status_word, void* stream) {
+                                       void* workspace, size_t workspace_bytes, int* status_word, void* stream) {
   PagedPrefillParams p = {};
   if (const int rc = daisy_host::paged_cache(cache, D, &p.c); rc != DAISY_OK) return rc;
-  if (!q || !lens || !out || !workspace || !tickets || B <= 0 || T <= 0 || Hq <= 0 || Hq % cache->H || !(scale > 0.f)) return DAISY_EINVAL;
+  if (!q || !lens || !out || !workspace || B <= 0 || T <= 0 || Hq <= 0 || Hq % cache->H || !(scale > 0.f)) return DAISY_EINVAL;
   if (flags & ~(DAISY_BOUNDED_QK | DAISY_CACHE_FP16)) return DAISY_EINVAL;
   if (B != (cu ? 1 : cache->n_seq)) return DAISY_EINVAL;
   if (!daisy_aligned16(q) || !daisy_aligned16(out) || ((q_sb | q_st | q_sh | o_sb | o_st | o_sh) & 7) || (reinterpret_cast<uintptr_t>(lens) & 3) ||
-      (reinterpret_cast<uintptr_t>(cu) & 3) || (reinterpret_cast<uintptr_t>(tickets) & 3) || (reinterpret_cast<uintptr_t>(workspace) & 255))
+      (reinterpret_cast<uintptr_t>(cu) & 3) || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return DAISY_EALIGN;
   // a zero stride on a dimension longer than 1 is a broadcast view, which the tile loads cannot express
   if ((T > 1 && q_st <= 0) || (Hq > 1 && q_sh <= 0) || (B > 1 && q_sb <= 0)) return DAISY_EINVAL;
   const int sms = daisy_host::sm_count_cached();
   if (sms <= 0) return DAISY_ENODEV;
   const int64_t tokens = (int64_t)B * T;
-  p.rows = prefill_rows(sms, tokens, cache->n_seq, Hq);
-  const PrefillRoom room = prefill_room(sms, tokens, cache->n_seq, p.rows);
+  p.G = Hq / cache->H;
+  p.lgp = prefill_lgp(p.G);
+  p.heads = Hq >> p.lgp;
+  p.window = window > 0 ? window : 0;
+  int64_t longest = ((int64_t)cache->width * cache->page + PP_BN - 1) / PP_BN;
+  if (p.window > 0) longest = std::min<int64_t>(longest, ((int64_t)p.window + (2 * PP_BM >> p.lgp)) / PP_BN + 2);
+  p.toks = prefill_toks(sms, tokens, cache->n_seq, Hq, p.lgp, longest);
+  const PrefillRoom room = prefill_room(sms, tokens, cache->n_seq, p.toks);
   if (workspace_bytes < room.end) return DAISY_EWORKSPACE;
   if ((room.max_pieces + 1) * Hq >= ((int64_t)1 << 31) - 4096) return DAISY_EUNSUPPORTED;
   if (const int rc = paged_prefill_smem(); rc != DAISY_OK) { (void)cudaGetLastError(); return rc; }
@@ -825,32 +918,42 @@ extern "C" int daisy_b200_paged_attend(const daisy_b200_pages* cache, const void
   auto sb = [](int64_t s, int64_t n) { return (uint64_t)(n == 1 ? 16 : s * 2); };
   int rc;
   const uint32_t box = (uint32_t)(cache->page < PP_BN ? cache->page : PP_BN);
-  if ((rc = daisy_host::make_tmap_bf16_dthb(&tq, q, D, T, Hq, B, sb(q_st, T), sb(q_sh, Hq), sb(q_sb, B), 64, PP_BM)) != DAISY_OK) return rc;
+  if ((rc = make_tmap_packed_rows(&tq, q, D, Hq, T, B, sb(q_sh, Hq), sb(q_st, T), sb(q_sb, B), 1u << p.lgp, (uint32_t)(PP_BM >> p.lgp))) != DAISY_OK) return rc;
   if ((rc = daisy_host::make_tmap_bf16_dthb(&tk, cache->k, D, cache->page, cache->H, cache->n_pages, cache->p_sr * 2, sb(cache->p_sh, cache->H),
                                             sb(cache->p_sb, cache->n_pages), 64, box)) != DAISY_OK) return rc;
   if ((rc = daisy_host::make_tmap_bf16_dthb(&tv, cache->v, D, cache->page, cache->H, cache->n_pages, cache->p_sr * 2, sb(cache->p_sh, cache->H),
                                             sb(cache->p_sb, cache->n_pages), 64, box)) != DAISY_OK) return rc;
   p.out = (__nv_bfloat16*)out; p.o_sb = o_sb; p.o_st = o_st; p.o_sh = o_sh;
   p.lens = lens; p.cu = cu;
-  p.T = T; p.Hq = Hq; p.G = Hq / cache->H; p.window = window > 0 ? window : 0;
+  p.T = T; p.Hq = Hq;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = status_word;
   char* ws = (char*)workspace;
-  p.tickets = tickets;
-  p.head = (PlanHead*)(ws + room.head);
+  p.head = (PlanHead*)ws;
   p.pieces = (Piece*)(ws + room.pieces);
+  p.cuts = (Cut*)(ws + room.cuts);
   p.part = (float*)(ws + room.part);
   p.slots = room.slots; p.max_pieces = (int)room.max_pieces;
   cudaStream_t st = (cudaStream_t)stream;
   const bool f16 = (flags & DAISY_CACHE_FP16) != 0;
   // weights without a reference maximum reach 2^60, which float16 does not hold
   const bool bounded = (flags & DAISY_BOUNDED_QK) && !f16 && scale * 1.4426950408889634f * (float)D <= 60.f;
-  cudaError_t e = daisy_host::launch_dependent(paged_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, p, sms);
+  // No plan where all sequences have as many queries and tables, or windows, are too short for items of uneven length: 131 tokens x 6 heads
+  // 17.5 us with it, 9.9 without
+  const int64_t per_seq = (T + p.toks - 1) / p.toks, items = per_seq * cache->n_seq * p.heads;
+  if (!cu && longest <= PP_SHORT) p.counted = (int)per_seq;
+  // Cutting pays where items are fewer than three a SM
+  if (tokens / p.toks * p.heads >= 3 * (int64_t)sms) p.slots = 0;
+  cudaError_t e = cudaSuccess;
+  if (!p.counted) e = daisy_host::launch_dependent(paged_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, p, sms);
+  const dim3 grid((unsigned)(p.counted ? std::min<int64_t>(items, sms) : sms));
   if (e == cudaSuccess) {
-    if (bounded)  e = daisy_host::launch_dependent(paged_prefill_kernel<2, false>, dim3(sms), dim3(576), PP_SMEM, st, tq, tk, tv, p);
-    else if (f16) e = daisy_host::launch_dependent(paged_prefill_kernel<1, true>, dim3(sms), dim3(320), PP_SMEM, st, tq, tk, tv, p);
-    else          e = daisy_host::launch_dependent(paged_prefill_kernel<1, false>, dim3(sms), dim3(320), PP_SMEM, st, tq, tk, tv, p);
+    if (bounded)  e = daisy_host::launch_dependent(paged_prefill_kernel<2, false>, grid, dim3(576), PP_SMEM, st, tq, tk, tv, p);
+    else if (f16) e = daisy_host::launch_dependent(paged_prefill_kernel<1, true>, grid, dim3(320), PP_SMEM, st, tq, tk, tv, p);
+    else          e = daisy_host::launch_dependent(paged_prefill_kernel<1, false>, grid, dim3(320), PP_SMEM, st, tq, tk, tv, p);
   }
+  if (e == cudaSuccess && !p.counted && p.slots > 0)
+    e = bounded ? daisy_host::launch_dependent(paged_join_kernel<2>, dim3(sms * 4), dim3(256), 0, st, p) : daisy_host::launch_dependent(paged_join_kernel<1>, dim3(sms * 4), dim3(256), 0, st, p);
   if (e != cudaSuccess) { (void)cudaGetLastError(); return DAISY_ECUDA; }
   DAISY_CHECK_LAUNCH();
   return DAISY_OK;

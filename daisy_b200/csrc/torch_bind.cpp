@@ -109,7 +109,7 @@ void release_workspaces() {
   std::lock_guard<std::mutex> lock(g_mutex);
   g_pool.clear();
 }
-enum { WS_TOKEN = 0, WS_KDA_TOKEN = 1, WS_PAGED_DECODE = 2, WS_PAGED_ATTEND = 3 };
+enum { WS_TOKEN = 0, WS_KDA_TOKEN = 1, WS_PAGED_DECODE = 2 };
 
 // ------------------------------------------------------------------ decode step
 void rope_table(const Tensor& t, const char* name) {
@@ -1071,11 +1071,10 @@ Tensor paged_attend(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
   }
   if (T == 0) return out;
   checked_int(B * T, "q");
-  const Tensor ws = at::empty({(int64_t)daisy_b200_paged_attend_workspace_bytes((int)B, (int)T, c.n_seq, (int)checked_int(Hq, "q"))}, q.options().dtype(at::kByte));
-  const Tensor tickets = stream_workspace(q, WS_PAGED_ATTEND, (int64_t)daisy_b200_paged_attend_ticket_bytes());
+  const Tensor ws = at::empty({(int64_t)daisy_b200_paged_attend_workspace_bytes((int)B, (int)T, c.n_seq, (int)checked_int(Hq, "q"), c.H)}, q.options().dtype(at::kByte));
   check(daisy_b200_paged_attend(&c, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), len, cup, (int)std::min<int64_t>(std::max<int64_t>(window, 0), INT32_MAX), out.data_ptr(),
                                 out.stride(0), out.stride(1), out.stride(2), (int)B, (int)T, (int)Hq, 128, (float)scale,
-                                (bounded ? DAISY_BOUNDED_QK : 0) | (f16 ? DAISY_CACHE_FP16 : 0), ws.data_ptr(), (size_t)ws.numel(), (int32_t*)tickets.data_ptr(), status_ptr(q),
+                                (bounded ? DAISY_BOUNDED_QK : 0) | (f16 ? DAISY_CACHE_FP16 : 0), ws.data_ptr(), (size_t)ws.numel(), status_ptr(q),
                                 stream_of(q)),
         "daisy_b200_paged_attend");
   return out;

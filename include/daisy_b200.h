@@ -616,17 +616,15 @@ int daisy_b200_paged_decode_step(const daisy_b200_pages* cache, const void* q_ne
  *   out        [B,T,Hq,D] bf16, strides (o_sb,o_st,o_sh); rows of idle or refused sequences (fewer tokens than queries, more
  *              than the table holds) are zero, rows of nobody's tokens are left as they were
  *   flags      DAISY_BOUNDED_QK as in daisy_b200_swa_attend | DAISY_CACHE_FP16
- *   workspace  daisy_b200_paged_attend_workspace_bytes(B,T,n_seq,Hq) bytes on the current device (80 MB and the list of work
- *              items), 256-byte aligned, scratch
- *   tickets    daisy_b200_paged_attend_ticket_bytes() bytes, zero before the first call, afterwards left to the calls
- * Calls that may overlap on the device need both of their own.  Two launches: one block lists the work, then the attention. */
-size_t daisy_b200_paged_attend_workspace_bytes(int B, int T, int n_seq, int Hq);
-size_t daisy_b200_paged_attend_ticket_bytes(void);
+ *   workspace  daisy_b200_paged_attend_workspace_bytes(B,T,n_seq,Hq,H) bytes on the current device (80 MB and the list of work
+ *              items), 256-byte aligned, scratch; calls that may overlap on the device need workspaces of their own
+ * One to three launches: one block lists the work (where lengths may be uneven), the attention, the join of what was cut. */
+size_t daisy_b200_paged_attend_workspace_bytes(int B, int T, int n_seq, int Hq, int H);
 int daisy_b200_paged_attend(const daisy_b200_pages* cache, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
                             const int32_t* lens, const int32_t* cu, int window,
                             void* out, int64_t o_sb, int64_t o_st, int64_t o_sh,
                             int B, int T, int Hq, int D, float scale, unsigned flags,
-                            void* workspace, size_t workspace_bytes, int32_t* tickets, int* status_word, void* stream);
+                            void* workspace, size_t workspace_bytes, int* status_word, void* stream);
 
 #ifdef __cplusplus
 }
