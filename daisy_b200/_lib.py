@@ -95,6 +95,9 @@ SIGNATURES = {
                                      [_i] * 2 + [_f, _f, _u, _vp, _sz, _vp, _vp]),
     "daisy_b200_paged_attend_workspace_bytes": (_sz, [_i] * 5),
     "daisy_b200_paged_attend": (_i, [_vp] * 2 + [_i64] * 3 + [_vp] * 2 + [_i, _vp] + [_i64] * 3 + [_i] * 4 + [_f, _u, _vp, _sz] + [_vp] * 2),
+    "daisy_b200_paged_attend_few_rows": (_i, [_i] * 5),
+    "daisy_b200_paged_attend_few_workspace_bytes": (_sz, [_i] * 3),
+    "daisy_b200_paged_attend_few": (_i, [_vp] * 2 + [_i64] * 3 + [_vp] * 2 + [_i, _vp] + [_i64] * 3 + [_i] * 4 + [_f, _u, _vp, _sz] + [_vp] * 2),
 }
 
 

@@ -14,6 +14,9 @@
 // four.  Queries and weights go in as sums of two 16-bit values (two products each): scores and weights keep 16 bits and more.
 #include "paged.cuh"
 
+//
+// FEW: a few queries of every sequence instead of one (drafted tokens), prepared, their keys and values in the pages already; the
+// columns of a product are then (query, head) pairs, 8 a pass, each with its own last key.
 namespace daisy {
 
 constexpr int PD_WARPS = 4;
@@ -25,10 +28,12 @@ struct PagedDecodeParams {
   const __nv_bfloat16 *q, *k, *v, *ve;
   int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh, ve_sb, ve_sh, o_sb, o_sh;
   __nv_bfloat16* out;
-  const int* lens;
+  const int *lens, *cu;
   const float *cos, *sin, *ve_gate;
-  int window, table_rows, Hq, G;     // G query heads of one key head; they come in n_grp groups of at most 8 NT
+  int window, table_rows, Hq, G;     // G query heads of one key head; columns (heads, or queries x heads) come in up to n_grp groups of 8 NT
   int n_grp;
+  int T;                             // FEW: queries of a sequence, or of the packed row; q_st, o_st: from query to query
+  int64_t q_st, o_st;
   float qscale, eps;
   unsigned flags;
   int* status;
@@ -39,23 +44,50 @@ constexpr int PD_PART = 132;
 // What a pair costs beside its rows (queries, sums of the warps, the token's own row, output), in blocks of 64 rows: the deal counts it
 // as so many blocks without rows in front of the pair's.
 constexpr int PD_HEAD = 2;
+// FEW: columns (queries x heads of a key head) that one pass over the rows serves, and the most of a packed call: four passes where one
+// sequence has them all.  8 sequences of 9000 rows x 16 heads: 4 queries 97 us here, 121 on tcgen05 (paged_prefill.cu); 16 queries in one
+// pass of 16 columns 139, 121 there.
+constexpr int PD_FEW = 8, PD_FEW_PACKED = 32;
 constexpr int PD_JOIN = 16;          // shares that one CTA joins
 constexpr __host__ __device__ int pd_ctas(int cols) { return cols == 8 ? 3 : 2; }              // CTAs a SM, by registers
 
-// Where a sequence stands: its cached length, or -1 if it is idle or cannot have the position; rows lo .. len-1 are seen.
-struct SeqRange { int len, lo, tile0, tiles, blocks; };              // blocks: PD_HEAD, then one for every PD_WARPS tiles, the last one maybe short
-__device__ __forceinline__ int seq_len(const PagedDecodeParams& p, int b) { return __ldcg(p.lens + b); }   // L2: this grid may have been there before they were written
-__device__ __forceinline__ SeqRange seq_range(const PagedDecodeParams& p, int len) {
+// Where a sequence stands: its cached length, or -1 if it is idle or cannot have the position; rows lo .. len-1 are seen by some query.
+// blocks: PD_HEAD, then one for every PD_WARPS tiles, the last one maybe short.  FEW: n queries from row row0 of q, the first at position pos0.
+struct SeqRange { int len, lo, tile0, tiles, blocks, n, row0, pos0; };
+struct SeqIndex { int len, first, end; };                            // as the index arrays say; FEW: its queries first .. end - 1 of the row
+template <bool FEW>
+__device__ __forceinline__ SeqIndex seq_index(const PagedDecodeParams& p, int b) {          // L2: this grid may have been there before they were written
+  SeqIndex i{__ldcg(p.lens + b), 0, FEW ? p.T : 1};
+  if (FEW && p.cu) { i.first = __ldcg(p.cu + b); i.end = __ldcg(p.cu + b + 1); }
+  return i;
+}
+template <bool FEW>
+__device__ __forceinline__ SeqRange seq_range(const PagedDecodeParams& p, const SeqIndex& i) {
   SeqRange r;
-  r.len = len;
-  const bool bad = r.len >= p.c.capacity() || ((p.flags & DAISY_ROPE) && r.len >= p.table_rows);
+  r.len = i.len;
+  bool bad;
+  if (FEW) {
+    const bool sane = i.first >= 0 && i.end >= i.first && i.end <= p.T;                      // offsets outside the row: no queries
+    r.n = sane ? i.end - i.first : 0;
+    r.row0 = sane ? i.first : 0;
+    bad = !sane || (r.n > 0 && r.len >= 0 && (r.len < r.n || r.len > p.c.capacity()));
+  } else {
+    r.n = 1; r.row0 = 0;
+    bad = r.len >= p.c.capacity() || ((p.flags & DAISY_ROPE) && r.len >= p.table_rows);
+  }
   if (bad && p.status) p.status[0] = DAISY_EINVAL;
   if (r.len < 0 || bad) r.len = -1;
-  r.lo = p.window > 0 && r.len > p.window - 1 ? r.len - (p.window - 1) : 0;
+  r.pos0 = FEW ? r.len - r.n : r.len;
+  r.lo = p.window > 0 && r.pos0 > p.window - 1 ? r.pos0 - (p.window - 1) : 0;
   r.tile0 = r.lo / PD_TILE;
   r.tiles = r.len <= r.lo ? 1 : (r.len + PD_TILE - 1) / PD_TILE - r.tile0;      // one without rows: the token alone
   r.blocks = PD_HEAD + (r.tiles + PD_WARPS - 1) / PD_WARPS;
   return r;
+}
+// (key head, group of columns) pairs of a sequence
+template <bool FEW>
+__device__ __forceinline__ int pairs_of(const PagedDecodeParams& p, const SeqRange& r, int cols) {
+  return p.c.H * (FEW ? (r.n * p.G + cols - 1) / cols : p.n_grp);
 }
 
 template <bool F16>
@@ -100,22 +132,27 @@ __device__ __forceinline__ void row_of_warp(const __nv_bfloat16* src, bool norm,
   }
 }
 
-// Lengths of the first PD_KEPT sequences stay in shared memory.
+// Index entries of the first PD_KEPT sequences stay in shared memory.
 constexpr int PD_KEPT = 32 * PD_WARPS;
-struct DealSmem { int warp_sum[PD_WARPS]; int before, b; int len[PD_KEPT]; };
+struct DealSmem { int warp_sum[PD_WARPS]; int before, b; SeqIndex kept[PD_KEPT]; };
 
 // This CTA's run of blocks [t, t_end) of the batch, the sequence b that holds t, and where b's blocks begin.  The whole block calls it.
 struct Deal { int t, t_end, share, b_at, b; };
-__device__ __forceinline__ Deal deal_tiles(const PagedDecodeParams& p, int HH, DealSmem* sm) {
+template <bool FEW>
+__device__ __forceinline__ Deal deal_tiles(const PagedDecodeParams& p, int cols, DealSmem* sm) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Deal d;
   int base, x, t, total = 0;
-  // blocks (of one head) of sequences b0 .. b0 + PD_KEPT - 1: this thread's, their inclusive prefix sum, what lies in front of its warp
+  // blocks of sequences b0 .. b0 + PD_KEPT - 1: this thread's, their inclusive prefix sum, what lies in front of its warp
   auto scan = [&](int b0) {
     const int b = b0 + threadIdx.x;
-    const int len = b < p.c.n_seq ? seq_len(p, b) : -1;
-    if (b0 == 0) sm->len[threadIdx.x] = len;
-    x = t = b < p.c.n_seq ? seq_range(p, len).blocks : 0;
+    x = t = 0;
+    if (b < p.c.n_seq) {
+      const SeqIndex at = seq_index<FEW>(p, b);
+      if (b0 == 0) sm->kept[threadIdx.x] = at;
+      const SeqRange r = seq_range<FEW>(p, at);
+      x = t = r.blocks * pairs_of<FEW>(p, r, cols);
+    }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
@@ -136,13 +173,12 @@ __device__ __forceinline__ Deal deal_tiles(const PagedDecodeParams& p, int HH, D
     __syncthreads();
     total += scan(b0);
   }
-  total *= HH;
   d.share = (int)(((unsigned)total + gridDim.x - 1) / gridDim.x);
   d.t = min((unsigned)blockIdx.x * (unsigned)d.share, (unsigned)total);
   d.t_end = (int)min((unsigned)d.t + (unsigned)d.share, (unsigned)total);
   d.b = -1;
   if (d.t >= d.t_end) return d;
-  const int want = d.t / HH;
+  const int want = d.t;
   int front = 0;
   for (int b0 = 0; b0 < p.c.n_seq; b0 += PD_KEPT) {
     int sum = first_sum;
@@ -156,7 +192,7 @@ __device__ __forceinline__ Deal deal_tiles(const PagedDecodeParams& p, int HH, D
   }
   __syncthreads();
   d.b = sm->b;
-  d.b_at = sm->before * HH;
+  d.b_at = sm->before;
   return d;
 }
 
@@ -248,7 +284,7 @@ __device__ __forceinline__ void own_row(const PagedDecodeParams& p, int b, int h
   }
 }
 
-template <int NT, bool F16>
+template <int NT, bool F16, bool FEW>
 __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
   constexpr int NQ = 8 * NT;                                         // query heads of a pass, the last ones maybe absent
   __shared__ DealSmem sm_deal;
@@ -258,30 +294,37 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
   __shared__ OwnRow sm_own;
   __shared__ int sm_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int HH = p.c.H * p.n_grp;                                    // pairs a sequence
   grid_dep_launch();
   grid_dep_wait();
 
-  const Deal deal = deal_tiles(p, HH, &sm_deal);                     // pairs are (sequence, head)-major
+  const Deal deal = deal_tiles<FEW>(p, NQ, &sm_deal);                // pairs are (sequence, head)-major
   if (deal.b < 0) return;
   const int t_end = deal.t_end, share = deal.share;
   int t = deal.t, b_at = deal.b_at;
   int b = deal.b;
-  auto range_of = [&](int i) { return seq_range(p, i < PD_KEPT ? sm_deal.len[i] : seq_len(p, i)); };
+  auto range_of = [&](int i) { return seq_range<FEW>(p, i < PD_KEPT ? sm_deal.kept[i] : seq_index<FEW>(p, i)); };
   SeqRange r = range_of(b);
 
   while (t < t_end) {
-    while (t >= b_at + r.blocks * HH) {
+    while (t >= b_at + r.blocks * pairs_of<FEW>(p, r, NQ)) {
       if (b + 1 >= p.c.n_seq) return;                                // lengths that changed under the call
-      b_at += r.blocks * HH;
+      b_at += r.blocks * pairs_of<FEW>(p, r, NQ);
       r = range_of(++b);
     }
-    const int hh = (t - b_at) / r.blocks, h = hh / p.n_grp, grp = hh % p.n_grp;
+    const int n_grp = FEW ? (r.n * p.G + NQ - 1) / NQ : p.n_grp;
+    const int hh = (t - b_at) / r.blocks, h = hh / n_grp, grp = hh % n_grp;
     const int u_at = b_at + hh * r.blocks;                           // this pair's blocks: u_at .. u_end - 1
     const int u_end = u_at + r.blocks, s_end = min(u_end, t_end);
     const int r_at = max(t, u_at + PD_HEAD);                         // this CTA's blocks with rows: r_at .. s_end - 1
     if (r_at >= s_end) { t = s_end; continue; }
-    const int q_h0 = h * p.G + grp * NQ, n_q = min(NQ, p.G - grp * NQ);
+    const int q_h0 = h * p.G + grp * NQ, n_q = min(NQ, (FEW ? r.n * p.G : p.G) - grp * NQ);
+    // FEW: column -> query of the sequence
+    auto query_of = [&](int col) { return (grp * NQ + col) / p.G; };
+    auto q_at = [&](int col) -> const __nv_bfloat16* {
+      if (!FEW) return p.q + b * p.q_sb + (q_h0 + col) * p.q_sh;
+      const int i = query_of(col);
+      return p.q + (p.cu ? 0 : b) * p.q_sb + (int64_t)(r.row0 + i) * p.q_st + (h * p.G + grp * NQ + col - i * p.G) * p.q_sh;
+    };
     const float *cos_row = p.cos + (int64_t)max(r.len, 0) * 64, *sin_row = p.sin + (int64_t)max(r.len, 0) * 64;
 
     // what the queries are made of is asked for first: the table's entry and the rows behind it take longer
@@ -291,7 +334,8 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        q_raw[n][j] = 8 * n + g < n_q ? ld_cg16(p.q + b * p.q_sb + (q_h0 + 8 * n + g) * p.q_sh + 32 * j + 8 * c) : make_uint4(0, 0, 0, 0);
+        q_raw[n][j] = 8 * n + g < n_q ? ld_cg16(q_at(8 * n + g) + 32 * j + 8 * c) : make_uint4(0, 0, 0, 0);
+    if constexpr (!FEW)
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -318,6 +362,12 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
     const int64_t sr = 2 * p.c.p_sr;
     auto seen = [&](int row) { return row >= r.lo && row < r.len; };
     auto whole = [&](int tile) { return tile * PD_TILE >= r.lo && tile * PD_TILE + PD_TILE <= r.len; };
+    int q_pos[NT][2];                                                // FEW: positions of this lane's columns
+    if constexpr (FEW)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) { q_pos[n][0] = r.pos0 + query_of(8 * n + 2 * c); q_pos[n][1] = r.pos0 + query_of(8 * n + 2 * c + 1); }
+    // the first position that all queries see, and the last
+    const int all_lo = FEW && p.window > 0 ? max(r.lo, r.len - p.window) : r.lo, all_hi = FEW ? r.pos0 : r.len - 1;
     auto fetch_k = [&](int tile, int pg, uint4 (&kk)[2][4]) {
       const char* kb = p.c.k + p.c.at(pg, h, tile * PD_TILE) + 16 * c;
       if (whole(tile)) {
@@ -367,7 +417,16 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
     for (int n = 0; n < NT; ++n) {
       float x[4][8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) unpack8(q_raw[n][j], x[j]);
+      for (int j = 0; j < 4; ++j) {
+        if (FEW) {                                                   // prepared, in the pages' type
+          const uint32_t u[4] = {q_raw[n][j].x, q_raw[n][j].y, q_raw[n][j].z, q_raw[n][j].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { const float2 f = unpack16<F16>(u[i]); x[j][2 * i] = f.x * p.qscale; x[j][2 * i + 1] = f.y * p.qscale; }
+        } else {
+          unpack8(q_raw[n][j], x[j]);
+        }
+      }
+      if constexpr (!FEW) {
       float mul = p.qscale;
       if (p.flags & DAISY_NORM_Q) {
         float ss = 0.f;
@@ -390,9 +449,9 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
           x[j + 2][e] = d * cs[e] - a * sn[e];
         }
       }
+      }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-      {
+      for (int j = 0; j < 4; ++j) {
         uint32_t lo[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -434,7 +493,16 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
             mma16816<F16>(s[n], k0[i], k1[i], k0[i + 1], k1[i + 1], i ? ql[n].z : ql[n].x, i ? ql[n].w : ql[n].y);
           }
       }
-      if (!whole(tile)) {
+      if constexpr (FEW) {
+        if (row0 < all_lo || row0 + PD_TILE - 1 > all_hi) {
+          auto hidden = [&](int key, int pos) { return key > pos || (p.window > 0 && key <= pos - p.window); };
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (hidden(row0 + g + 8 * (i >> 1), q_pos[n][i & 1])) s[n][i] = -INFINITY;
+        }
+      } else if (!whole(tile)) {
         const bool in0 = seen(row0 + g), in1 = seen(row0 + g + 8);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -538,12 +606,12 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
     if (threadIdx.x == 0) {
       sm_last = 1;
       if (!alone) {                                                  // of the group's shares, or of the pair's where there is one group
-        int* tk = n_grps > 1 ? p.tickets_grp + place(c_grp) : p.tickets + ((int64_t)b * HH + hh);
+        int* tk = n_grps > 1 ? p.tickets_grp + place(c_grp) : p.tickets + ((int64_t)b * p.c.H * p.n_grp + hh);
         const int of = min(c_grp + PD_JOIN - 1, c1) - c_grp;
         sm_last = atomicAdd(tk, 1) == of;
         if (sm_last) *tk = 0;                                        // every other one has been drawn
       }
-    } else if (warp > 0 && r.len >= 0) {
+    } else if (!FEW && warp > 0 && r.len >= 0) {
       own_row<F16>(p, b, h, q_h0, n_q, r.len, &sm_own, sm_self);
     }
     __syncthreads();
@@ -563,7 +631,7 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
-        int* tk = p.tickets + ((int64_t)b * HH + hh);
+        int* tk = p.tickets + ((int64_t)b * p.c.H * p.n_grp + hh);
         sm_last = atomicAdd(tk, 1) == n_grps - 1;
         if (sm_last) *tk = 0;
       }
@@ -576,7 +644,7 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
       }
     }
     if (finish) {
-      if (warp == PD_WARPS - 1 && grp == 0 && r.len >= 0) {
+      if (!FEW && warp == PD_WARPS - 1 && grp == 0 && r.len >= 0) {
         if ((unsigned)sm_own.page < (unsigned)p.c.n_pages) {
           const int64_t at = p.c.at(sm_own.page, h, r.len) + 8 * lane;
           *reinterpret_cast<uint2*>(p.c.k + at) = sm_own.k16[lane];
@@ -589,12 +657,23 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
         if (r.len >= 0) {
           const Sums x = mine(col);
-          const float self = sm_self[col], top = fmaxf(x.ref, self), a = fast_exp2(x.ref - top), w = fast_exp2(self - top);
-          const float4 v = sm_own.v[lane];
-          const float inv = 1.0f / (x.den * a + w), ai = a * inv, wi = w * inv;
-          y = make_float4(x.num.x * ai + wi * v.x, x.num.y * ai + wi * v.y, x.num.z * ai + wi * v.z, x.num.w * ai + wi * v.w);
+          if (FEW) {
+            const float inv = 1.0f / x.den;
+            y = make_float4(x.num.x * inv, x.num.y * inv, x.num.z * inv, x.num.w * inv);
+          } else {
+            const float self = sm_self[col], top = fmaxf(x.ref, self), a = fast_exp2(x.ref - top), w = fast_exp2(self - top);
+            const float4 v = sm_own.v[lane];
+            const float inv = 1.0f / (x.den * a + w), ai = a * inv, wi = w * inv;
+            y = make_float4(x.num.x * ai + wi * v.x, x.num.y * ai + wi * v.y, x.num.z * ai + wi * v.z, x.num.w * ai + wi * v.w);
+          }
         }
-        __nv_bfloat16* dst = p.out + b * p.o_sb + (q_h0 + col) * p.o_sh + 4 * lane;
+        __nv_bfloat16* dst = p.out + 4 * lane;
+        if (FEW) {
+          const int i = query_of(col);
+          dst += (p.cu ? 0 : b) * p.o_sb + (int64_t)(r.row0 + i) * p.o_st + (h * p.G + grp * NQ + col - i * p.G) * p.o_sh;
+        } else {
+          dst += b * p.o_sb + (q_h0 + col) * p.o_sh;
+        }
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
       }
     }
@@ -667,8 +746,61 @@ extern "C" int daisy_b200_paged_decode_step(const daisy_b200_pages* cache, const
   const bool f16 = (flags & DAISY_CACHE_FP16) != 0;
   cudaStream_t st = (cudaStream_t)stream;
   auto go = [&](auto kernel) { return daisy_host::launch_dependent(kernel, dim3(grid), dim3(32 * PD_WARPS), 0, st, p); };
-  const cudaError_t e = nq == 8 ? (f16 ? go(paged_decode_kernel<1, true>) : go(paged_decode_kernel<1, false>))
-                                : (f16 ? go(paged_decode_kernel<2, true>) : go(paged_decode_kernel<2, false>));
+  const cudaError_t e = nq == 8 ? (f16 ? go(paged_decode_kernel<1, true, false>) : go(paged_decode_kernel<1, false, false>))
+                                : (f16 ? go(paged_decode_kernel<2, true, false>) : go(paged_decode_kernel<2, false, false>));
+  if (e != cudaSuccess) { (void)cudaGetLastError(); return DAISY_ECUDA; }
+  DAISY_CHECK_LAUNCH();
+  return DAISY_OK;
+}
+
+extern "C" int daisy_b200_paged_attend_few_rows(int T, int n_seq, int packed, int Hq, int H) {
+  if (T <= 0 || n_seq <= 0 || Hq <= 0 || H <= 0 || Hq % H) return 0;
+  const int64_t cols = (int64_t)T * (Hq / H);
+  // packed, the lengths are not known here: few tokens, and few a sequence
+  return packed ? (cols <= PD_FEW_PACKED && cols <= (int64_t)n_seq * (PD_FEW / 2) ? (int)cols : 0) : (cols <= PD_FEW ? (int)cols : 0);
+}
+
+extern "C" size_t daisy_b200_paged_attend_few_workspace_bytes(int n_seq, int H, int D) {
+  if (n_seq <= 0 || H <= 0 || D != DAISY_HEAD_DIM) return 0;
+  int sms = daisy_host::sm_count_cached();
+  if (sms <= 0) sms = daisy_host::MAX_SMS;
+  return partials_bytes(sms) + group_tickets_bytes(sms) + ((size_t)n_seq * H * (PD_FEW_PACKED / PD_FEW) * sizeof(int) + 15) / 16 * 16;
+}
+
+extern "C" int daisy_b200_paged_attend_few(const daisy_b200_pages* cache, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                                           const int32_t* lens, const int32_t* cu, int window,
+                                           void* out, int64_t o_sb, int64_t o_st, int64_t o_sh,
+                                           int B, int T, int Hq, int D, float scale, unsigned flags,
+                                           void* workspace, size_t workspace_bytes, int* status_word, void* stream) {
+  PagedDecodeParams p = {};
+  if (const int rc = daisy_host::paged_cache(cache, D, &p.c); rc != DAISY_OK) return rc;
+  if (!q || !lens || !out || !workspace || B <= 0 || T <= 0 || Hq <= 0 || Hq % cache->H || !(scale > 0.f)) return DAISY_EINVAL;
+  if (flags & ~(DAISY_BOUNDED_QK | DAISY_CACHE_FP16)) return DAISY_EINVAL;
+  if (B != (cu ? 1 : cache->n_seq)) return DAISY_EINVAL;
+  const int cols = daisy_b200_paged_attend_few_rows(T, cache->n_seq, cu != nullptr, Hq, cache->H);
+  if (cols == 0) return DAISY_EUNSUPPORTED;
+  if (!daisy_aligned16(q) || !daisy_aligned16(workspace) || ((q_sb | q_st | q_sh) & 7) || ((o_sb | o_st | o_sh) & 3) || (reinterpret_cast<uintptr_t>(out) & 7) ||
+      (reinterpret_cast<uintptr_t>(lens) & 3) || (reinterpret_cast<uintptr_t>(cu) & 3))
+    return DAISY_EALIGN;
+  if (workspace_bytes < daisy_b200_paged_attend_few_workspace_bytes(cache->n_seq, cache->H, D)) return DAISY_EWORKSPACE;
+  const int sms = daisy_host::sm_count_cached();
+  if (sms <= 0) return DAISY_ENODEV;
+  p.G = Hq / cache->H; p.Hq = Hq; p.T = T; p.cu = cu;
+  p.n_grp = (cols + PD_FEW - 1) / PD_FEW;
+  const int64_t blocks = (int64_t)cache->width * cache->page / (PD_TILE * PD_WARPS) + 2 + PD_HEAD, pairs = (int64_t)cache->n_seq * cache->H * p.n_grp;
+  if (pairs >= (int64_t)1 << 31 || blocks * pairs >= ((int64_t)1 << 31) - 65536) return DAISY_EUNSUPPORTED;
+  p.q = (const __nv_bfloat16*)q; p.q_sb = q_sb; p.q_st = q_st; p.q_sh = q_sh;
+  p.out = (__nv_bfloat16*)out; p.o_sb = o_sb; p.o_st = o_st; p.o_sh = o_sh;
+  p.lens = lens; p.window = window > 0 ? window : 0;
+  p.qscale = scale * 1.4426950408889634f;
+  p.status = status_word;
+  const unsigned grid = (unsigned)(sms * pd_ctas(PD_FEW));
+  p.part = (float*)workspace;
+  p.tickets_grp = (int*)((char*)workspace + partials_bytes(sms));
+  p.tickets = (int*)((char*)p.tickets_grp + group_tickets_bytes(sms));
+  const bool f16 = (flags & DAISY_CACHE_FP16) != 0;
+  auto go = [&](auto kernel) { return daisy_host::launch_dependent(kernel, dim3(grid), dim3(32 * PD_WARPS), 0, (cudaStream_t)stream, p); };
+  const cudaError_t e = f16 ? go(paged_decode_kernel<1, true, true>) : go(paged_decode_kernel<1, false, true>);
   if (e != cudaSuccess) { (void)cudaGetLastError(); return DAISY_ECUDA; }
   DAISY_CHECK_LAUNCH();
   return DAISY_OK;

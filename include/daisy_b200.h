@@ -626,6 +626,19 @@ int daisy_b200_paged_attend(const daisy_b200_pages* cache, const void* q, int64_
                             int B, int T, int Hq, int D, float scale, unsigned flags,
                             void* workspace, size_t workspace_bytes, int* status_word, void* stream);
 
+/* The same for a few queries of every sequence, split over the cached rows like daisy_b200_paged_decode_step: up to 8 (query, head)
+ * pairs of a key head a sequence, or packed rows of up to 32 in all and 4 a sequence on average.
+ *   few_rows   T * Hq / H where the call below takes it, 0 where daisy_b200_paged_attend is to
+ *   workspace  daisy_b200_paged_attend_few_workspace_bytes bytes, 16-byte aligned, zero before the first call, afterwards left to
+ *              the calls (it may be one workspace with daisy_b200_paged_decode_step) */
+int    daisy_b200_paged_attend_few_rows(int T, int n_seq, int packed, int Hq, int H);
+size_t daisy_b200_paged_attend_few_workspace_bytes(int n_seq, int H, int D);
+int daisy_b200_paged_attend_few(const daisy_b200_pages* cache, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                                const int32_t* lens, const int32_t* cu, int window,
+                                void* out, int64_t o_sb, int64_t o_st, int64_t o_sh,
+                                int B, int T, int Hq, int D, float scale, unsigned flags,
+                                void* workspace, size_t workspace_bytes, int* status_word, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
