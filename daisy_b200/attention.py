@@ -35,7 +35,7 @@ import torch.nn.functional as F
 from . import ops
 from ._native import ext
 from ._lib import WRITE_RING, NORM_Q, NORM_K, NORM_V, ROPE, QKV_DEFAULT
-from .kv_cache import B200KVCache
+from .kv_cache import B200KVCache, B200PagedKVCache
 
 
 @dataclass(frozen=True)
@@ -415,3 +415,32 @@ class B200CausalSelfAttention(nn.Module):
             ve_kw = dict(ve=ve.to(torch.bfloat16), ve_gate_logit=self.g_ve.detach().float().reshape(1))
         return ops.swa_decode_step_fused(q, k, v, kc, vc, int(t), cap, window, cos[pos], sin[pos], self.attn_scale,
                                          self.norm_eps, QKV_DEFAULT, write_ring=write_ring, return_new_kv=True, **ve_kw)
+
+    # ------------------------------------------------------------------ paged cache (sequences of uneven length)
+    def _paged_ve(self, ve: Optional[Tensor]):
+        if not self.receives_ve:
+            return {}
+        torch._assert(ve is not None, "ve must be provided when receives_ve=True")
+        return dict(ve=ve.to(torch.bfloat16), ve_gate_logit=self.g_ve.detach().float().reshape(1))
+
+    def prefill_paged(self, x: Tensor, ve: Optional[Tensor], cache: B200PagedKVCache, layer: int, table: Tensor, start: Tensor, lens: Tensor,
+                      window: Optional[int], cu_seqlens: Optional[Tensor] = None):
+        """Prompts, or the next pieces of prompts, of sequences in a paged cache: ``x [n,T,dim]``, or packed ``[1,T_total,dim]`` with
+        ``cu_seqlens``; ``table [n, entries]`` their rows of ``cache.table``, ``start`` / ``lens [n]`` (int32 on the device) their
+        tokens in the cache before and with this piece.  Stores the keys and values, returns ``y`` of ``x``'s shape."""
+        B, T = x.size(0), x.size(1)
+        q, k, v = self._project(x)
+        kp, vp = cache.layer(layer)
+        qp = ops.paged_append(k, v, kp, vp, table, start, self.rotary.cos, self.rotary.sin, cu_seqlens, q, self.norm_eps, QKV_DEFAULT, **self._paged_ve(ve))
+        y = ops.paged_attend(qp, kp, vp, table, lens, window, cu_seqlens, self.attn_scale, bounded_qk=True)      # q, k are RMS-normalised
+        return self._linear(y.view(B, T, self.m_dim), self.qkvo_w.detach()[3])
+
+    def step_paged(self, x: Tensor, ve: Optional[Tensor], cache: B200PagedKVCache, layer: int, window: Optional[int],
+                   workspace: Optional[Tensor] = None):
+        """One token of every slot of a paged cache, ``x [max_seqs,1,dim]``, at position ``cache.lens``; stores its key and value (the
+        caller advances the cache).  Free slots give zeros.  Nothing depends on host values: the call can be captured."""
+        q, k, v = self._project(x)
+        kp, vp = cache.layer(layer)
+        y = ops.paged_decode_step(q, k, v, kp, vp, cache.table, cache.lens, window, self.rotary.cos, self.rotary.sin, self.attn_scale, self.norm_eps,
+                                  QKV_DEFAULT, workspace=workspace, **self._paged_ve(ve))
+        return self._linear(y.view(x.size(0), 1, self.m_dim), self.qkvo_w.detach()[3])

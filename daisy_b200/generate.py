@@ -5,6 +5,8 @@ stack of attention layers: prefill fills the ring layer by layer from inside the
 ``bulk_write_packed`` would write, no copy pass); each step is one launch that takes every layer's ring in place (no
 per-layer chronological ``view`` copy, no separate ``write``) and advances once.
 Sampling, embeddings and the MLPs are outside this path; the runner works on hidden states.
+
+:class:`PagedRunner` does the same for sequences of uneven length that come and go, over a paged cache.
 """
 from __future__ import annotations
 
@@ -15,7 +17,8 @@ import torch
 from ._lib import QKV_DEFAULT, WRITE_RING
 from ._native import ext
 from .attention import B200CausalSelfAttention, WindowMask
-from .kv_cache import B200KVCache
+from . import ops
+from .kv_cache import B200KVCache, B200PagedKVCache
 
 
 class StepRunner:
@@ -132,3 +135,110 @@ class StepRunner:
             x, _, _ = a.step_ring(x, self.cache, i, pos, None, self.window)
         self.cache.advance()
         return x
+
+
+class PagedRunner:
+    """A stack of attention layers serving up to ``max_seqs`` sequences of uneven length over a paged cache: prompts (whole or in
+    pieces) of several sequences at a time, then one token of every sequence a step.  Pages that ``window`` has left are given back."""
+
+    def __init__(self, layers: Sequence[B200CausalSelfAttention], window: Optional[int], pages: int, max_seqs: int, max_len: int, page: int = 64,
+                 device="cuda", dtype=torch.bfloat16):
+        assert len(layers) > 0
+        self.layers = list(layers)
+        self.window = window
+        a = self.layers[0]
+        self.cache = B200PagedKVCache(len(self.layers), pages, a.num_heads, a.head_dim, max_seqs, max_len, device, dtype, page)
+        torch._assert(max_len <= a.rotary.cos.shape[0], "Rotary buffers too small")
+        self._graph = None
+
+    def add(self) -> int:
+        """A slot for a new sequence."""
+        return self.cache.claim()
+
+    def drop(self, slot: int) -> None:
+        """A sequence has ended."""
+        self.cache.release(slot)
+
+    def _forget(self, slots) -> None:
+        if self.window:
+            for slot in slots:                                     # the next token sees window - 1 rows
+                self.cache.forget(slot, self.cache.length[slot] - self.window + 1)
+
+    @torch.inference_mode()
+    def prefill(self, prompts: Sequence[torch.Tensor], slots: Sequence[int]) -> List[torch.Tensor]:
+        """``prompts[i] [T_i, dim]``: the next tokens of the sequence in ``slots[i]`` (none twice), through every layer; returns each one's
+        outputs."""
+        if len(set(slots)) != len(slots) or len(slots) != len(prompts):
+            raise ValueError("one prompt a slot, no slot twice")
+        c = self.cache
+        counts = [p.size(0) for p in prompts]
+        c.reserve(slots, counts)
+        before = [c.length[s] for s in slots]
+        ends = [0]
+        for n in counts:
+            ends.append(ends[-1] + n)
+        # table rows, start, lens, cu_seqlens: one copy to the device
+        n = len(slots)
+        ints = torch.tensor(list(slots) + before + [b + m for b, m in zip(before, counts)] + ends, dtype=torch.int32).to(c.device)
+        table = c.table.index_select(0, ints[:n])
+        start, lens, cu = ints[n:2 * n], ints[2 * n:3 * n], ints[3 * n:]
+        x = torch.cat(list(prompts))[None]
+        for i, a in enumerate(self.layers):
+            x = a.prefill_paged(x, None, c, i, table, start, lens, self.window, cu)
+        c.advance(slots, counts)
+        self._forget(slots)
+        return list(x[0].split(counts))
+
+    def _begin_step(self):
+        slots = [s for s, n in enumerate(self.cache.length) if n >= 0]
+        self.cache.reserve(slots, 1)
+        return slots
+
+    def _end_step(self, slots):
+        self.cache.book.advance(slots, [1] * len(slots))
+        if self.window:                                            # a page is left once in `page` tokens
+            self._forget([s for s in slots if (self.cache.length[s] - self.window + 1) % self.cache.page == 0])
+
+    @torch.inference_mode()
+    def step(self, x: torch.Tensor) -> torch.Tensor:
+        """One token of every sequence, ``x [max_seqs, 1, dim]`` by slot (rows of free slots are ignored) -> ``y`` of its shape."""
+        slots = self._begin_step()
+        for i, a in enumerate(self.layers):
+            x = a.step_paged(x, None, self.cache, i, self.window)
+        self.cache.lens += self.cache.active
+        self._end_step(slots)
+        return x
+
+    @torch.inference_mode()
+    def capture_step(self, dim: int) -> None:
+        """Record the step of all layers into a CUDA graph for :meth:`step_graph`.  Lengths and pages are read on the device, so one
+        recording serves whatever sequences come and go; it must be made while no slot is taken."""
+        c = self.cache
+        if any(n >= 0 for n in c.length):
+            raise RuntimeError("capture the step before the first sequence is added")
+        self._gx = torch.zeros(c.max_seqs, 1, dim, device=c.device, dtype=torch.bfloat16)
+        self._gws = ops.paged_decode_workspace(c.max_seqs, c.H, c.H, c.device)
+
+        def body():
+            x = self._gx
+            for i, a in enumerate(self.layers):
+                x = a.step_paged(x, None, c, i, self.window, workspace=self._gws)
+            c.lens += c.active
+            return x
+        side = torch.cuda.Stream(device=c.device)
+        side.wait_stream(torch.cuda.current_stream(c.device))
+        with torch.cuda.stream(side):                              # warm-up: all slots are free, nothing is stored
+            body()
+        torch.cuda.current_stream(c.device).wait_stream(side)
+        self._graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self._graph):
+            self._gy = body()
+
+    @torch.inference_mode()
+    def step_graph(self, x: torch.Tensor) -> torch.Tensor:
+        """:meth:`step` from the recording; the result is a fixed buffer, overwritten by the next call."""
+        slots = self._begin_step()
+        self._gx.copy_(x)
+        self._graph.replay()
+        self._end_step(slots)
+        return self._gy

@@ -6,8 +6,12 @@ lives in row ``p % W``, ``t`` counts committed tokens.  ``view`` / ``write`` /
 ``bulk_write_packed`` keep the reference's shapes and ordering; in addition ``ring(layer)``
 hands the in-place ring to the decode kernel so the per-token chronological copy that
 ``view`` makes once the ring has wrapped is never needed on the hot path.
+
+:class:`B200PagedKVCache` serves sequences of uneven length: one pool of pages instead of a ring per batch row.
 """
 from __future__ import annotations
+
+from typing import Iterable, List
 
 import torch
 
@@ -111,3 +115,139 @@ class B200KVCache:
     def mark_written(self, layer):
         """Record that the decode kernel stored the new row of ``layer`` itself."""
         self._staged[layer] = True
+
+
+class B200PagedKVCache:
+    """Keys and values of up to ``max_seqs`` sequences of uneven length in one pool of pages.
+
+    Storage ``k, v [L, pages, H, page, D]``; position ``p`` of the sequence in slot ``s`` lies in row ``p % page`` of page
+    ``table[s, p // page]`` (int32, -1: none).  ``lens [max_seqs]`` (int32 on the device, mirrored in ``length``) counts the
+    tokens in the cache, -1 marks a free slot.  The kernels (``ops.paged_append``, ``paged_decode_step``, ``paged_attend``) read both on
+    the device; the page bookkeeping is host arithmetic, with a copy to the device only where a row of the table changes."""
+
+    def __init__(self, L, pages, H, D, max_seqs, max_len, device, dtype=torch.bfloat16, page=64):
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise ValueError("B200PagedKVCache lives in GPU memory; daisy_b200 has no CPU path")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"pages hold bfloat16 or float16, not {dtype}")
+        if page not in (16, 32, 64, 128, 256):
+            raise ValueError(f"pages hold 16, 32, 64, 128 or 256 rows, got {page}")
+        self.L, self.pages, self.H, self.D = L, pages, H, D
+        self.max_seqs, self.max_len, self.page = max_seqs, max_len, page
+        self.device, self.dtype = dev, dtype
+        shape = (L, pages, H, page, D)
+        self.k = torch.zeros(shape, device=dev, dtype=dtype)
+        self.v = torch.zeros(shape, device=dev, dtype=dtype)
+        self.table = torch.full((max_seqs, -(-max_len // page)), -1, device=dev, dtype=torch.int32)
+        self.lens = torch.full((max_seqs,), -1, device=dev, dtype=torch.int32)
+        self.active = torch.zeros(max_seqs, device=dev, dtype=torch.int32)
+        self.book = PageBook(pages, max_seqs, max_len, page)
+
+    @property
+    def length(self) -> List[int]:
+        return self.book.length
+
+    def layer(self, layer):
+        """``(k, v)`` of one layer as ``[pages, H, page, D]`` views of the storage."""
+        return self.k[layer], self.v[layer]
+
+    def claim(self) -> int:
+        """A free slot for a new sequence, of length 0."""
+        slot = self.book.claim()
+        self.lens[slot] = 0
+        self.active[slot] = 1
+        return slot
+
+    def release(self, slot: int) -> None:
+        """Give a sequence's pages back and free its slot."""
+        self.book.release(slot)
+        self.table[slot] = -1
+        self.lens[slot] = -1
+        self.active[slot] = 0
+
+    def reserve(self, slots: Iterable[int], tokens) -> None:
+        """Pages for ``tokens`` (a number, or one for each slot) more tokens of every sequence; raises ``RuntimeError``, with
+        nothing changed, where the pool has too few."""
+        slots = list(slots)
+        counts = [tokens] * len(slots) if isinstance(tokens, int) else list(tokens)
+        self._store(self.book.reserve(slots, counts))
+
+    def forget(self, slot: int, before: int) -> None:
+        """Give back the pages that hold only positions below ``before`` (a window has moved past them)."""
+        self._store(self.book.forget(slot, before))
+
+    def advance(self, slots: Iterable[int], tokens) -> None:
+        """Count ``tokens`` (a number, or one for each slot) stored tokens."""
+        slots = list(slots)
+        counts = [tokens] * len(slots) if isinstance(tokens, int) else list(tokens)
+        self.book.advance(slots, counts)
+        self.lens.copy_(torch.tensor(self.book.length, dtype=torch.int32))
+
+    def _store(self, rows) -> None:
+        for slot in rows:
+            self.table[slot].copy_(torch.tensor(self.book.table[slot], dtype=torch.int32))
+
+
+class PageBook:
+    """Which pages belong to which sequence: the host side of :class:`B200PagedKVCache`, no tensors."""
+
+    def __init__(self, pages, max_seqs, max_len, page):
+        self.page, self.max_len = page, max_len
+        self.free = list(range(pages - 1, -1, -1))
+        self.length = [-1] * max_seqs
+        self.table = [[-1] * -(-max_len // page) for _ in range(max_seqs)]
+        self.first = [0] * max_seqs             # entries below have been given back
+        self.end = [0] * max_seqs               # entries from here on have no page yet
+
+    def claim(self):
+        if -1 not in self.length:
+            raise RuntimeError("all slots of the paged cache are taken")
+        slot = self.length.index(-1)
+        self.length[slot] = 0
+        return slot
+
+    def _check(self, slot):
+        if not 0 <= slot < len(self.length) or self.length[slot] < 0:
+            raise ValueError(f"slot {slot} holds no sequence")
+
+    def release(self, slot):
+        self._check(slot)
+        row = self.table[slot]
+        self.free.extend(row[self.first[slot]:self.end[slot]])
+        self.table[slot] = [-1] * len(row)
+        self.length[slot], self.first[slot], self.end[slot] = -1, 0, 0
+
+    def reserve(self, slots, counts):
+        want = {}
+        for slot, n in zip(slots, counts):
+            self._check(slot)
+            if n < 0 or self.length[slot] + n > self.max_len:
+                raise ValueError(f"slot {slot}: {self.length[slot]} + {n} tokens, the table holds {self.max_len}")
+            want[slot] = max(want.get(slot, 0), -(-(self.length[slot] + n) // self.page) - self.end[slot])
+        if sum(max(w, 0) for w in want.values()) > len(self.free):
+            raise RuntimeError(f"the paged cache has {len(self.free)} pages left")
+        changed = [slot for slot, w in want.items() if w > 0]
+        for slot in changed:
+            for _ in range(want[slot]):
+                self.table[slot][self.end[slot]] = self.free.pop()
+                self.end[slot] += 1
+        return changed
+
+    def forget(self, slot, before):
+        self._check(slot)
+        upto = min(max(before, 0) // self.page, self.end[slot])
+        if upto <= self.first[slot]:
+            return []
+        row = self.table[slot]
+        self.free.extend(row[self.first[slot]:upto])
+        row[self.first[slot]:upto] = [-1] * (upto - self.first[slot])
+        self.first[slot] = upto
+        return [slot]
+
+    def advance(self, slots, counts):
+        for slot, n in zip(slots, counts):
+            self._check(slot)
+            if n < 0 or self.length[slot] + n > self.end[slot] * self.page:
+                raise ValueError(f"slot {slot} has no pages for {n} more tokens")
+            self.length[slot] += n
