@@ -80,19 +80,22 @@ __device__ __forceinline__ int last_tile(int pos, int n) { return (pos + n - 1) 
 
 // The pieces of a call, longest first.  One block; a warp a sequence, a lane an item.
 // How far items are cut: into pieces of at most L tiles, L from a few candidates by the estimate
-// total / CTAs + half a longest piece, or a longest piece where all pieces find a CTA, and ten tiles' time for every piece of a cut item
-// (its sums are written, and read again by the last: 8192 tokens x 16 heads cut in halves 322 us, whole 278).
+// total / CTAs + half a piece such as come last (they go longest first: halfway between the shortest item and the mean), or a longest piece
+// where all pieces find a CTA, and PLAN_COST tiles' time for every piece of a cut item
+// (its sums are written, and read again by the last: 8192 tokens x 16 heads cut in halves 322 us, whole 278).  The last candidate cuts only
+// the shortest items, as many as whole rounds of all CTAs leave over, into as many pieces as find a CTA then (8192 queries x 16 heads over 65536
+// keys, 512 items: 3755 us whole, 3480 so).
 constexpr float PLAN_COST = 8.f;
-constexpr int PLAN_THREADS = 1024, PLAN_CAND = 6, PLAN_BUCKETS = 1024, PLAN_KEPT = 1024;
-struct PlanItem { int b, i0, j0, j1, pos, n, row0; };               // j1 < j0: queries that see nothing
+constexpr int PLAN_THREADS = 1024, PLAN_CAND = 6, PLAN_BUCKETS = 1024, PLAN_KEPT = 1024, PLAN_TAIL = 256;
+struct PlanItem { int b, i0, j0, j1, pos, n, row0, cut; };          // j1 < j0: queries that see nothing
 __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PagedPrefillParams p, int ctas) {
   __shared__ PlanItem kept[PLAN_KEPT];
   __shared__ int hist[PLAN_BUCKETS];
   __shared__ unsigned long long sm_total;
-  __shared__ int sm_longest, sm_items, sm_slots, sm_cuts, sm_cut, sm_pieces[PLAN_CAND], sm_parts[PLAN_CAND], sm_L[PLAN_CAND], warp_sums[32];
+  __shared__ int sm_longest, sm_shortest, sm_items, sm_slots, sm_cuts, sm_cut, sm_pieces[PLAN_CAND], sm_parts[PLAN_CAND], sm_L[PLAN_CAND], sm_tail, sm_tail_parts, warp_sums[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   hist[threadIdx.x] = 0;
-  if (threadIdx.x == 0) { sm_total = 0; sm_longest = 0; sm_items = 0; sm_slots = 0; sm_cuts = 0; }
+  if (threadIdx.x == 0) { sm_total = 0; sm_longest = 0; sm_shortest = 1 << 30; sm_items = 0; sm_slots = 0; sm_cuts = 0; }
   if (threadIdx.x < PLAN_CAND) { sm_pieces[threadIdx.x] = 0; sm_parts[threadIdx.x] = 0; }
   grid_dep_launch();
   grid_dep_wait();
@@ -103,7 +106,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PagedPre
       const SeqQueries s = seq_queries(p, b);
       if (s.refused && p.status && lane == 0) p.status[0] = DAISY_EINVAL;
       for (int i0 = lane * p.toks; i0 < s.n; i0 += 32 * p.toks) {
-        PlanItem it{b, i0, 1, 0, -1, min(p.toks, s.n - i0), s.row0 + i0};
+        PlanItem it{b, i0, 1, 0, -1, min(p.toks, s.n - i0), s.row0 + i0, 0};
         if (s.pos >= 0) { it.pos = s.pos + i0; it.j0 = first_tile(it.pos, p.window); it.j1 = last_tile(it.pos, it.n); }
         f(it);
       }
@@ -111,16 +114,18 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PagedPre
   };
   {
     unsigned total = 0;
-    int longest = 0;
+    int longest = 0, shortest = 1 << 30;
     count_off([&](const PlanItem& it) {
       const int at = atomicAdd(&sm_items, 1), t = it.j1 - it.j0 + 1;
       if (at < PLAN_KEPT) kept[at] = it;
       total += t;
       longest = max(longest, t);
+      shortest = min(shortest, t);
     });
     total = __reduce_add_sync(0xffffffffu, total);
     longest = __reduce_max_sync(0xffffffffu, longest);
-    if (lane == 0 && longest > 0) { atomicAdd(&sm_total, (unsigned long long)total); atomicMax(&sm_longest, longest); }
+    shortest = __reduce_min_sync(0xffffffffu, shortest);
+    if (lane == 0 && longest > 0) { atomicAdd(&sm_total, (unsigned long long)total); atomicMax(&sm_longest, longest); atomicMin(&sm_shortest, shortest); }
   }
   __syncthreads();
   const int n_items = sm_items;
@@ -130,7 +135,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PagedPre
   };
   if (threadIdx.x < PLAN_CAND) {
     const int fit = n_items > 0 ? ctas / max(1, n_items * p.heads) : 1;
-    const int n = threadIdx.x == 0 ? 1 : threadIdx.x == 1 ? max(1, fit) : threadIdx.x;             // whole; as many as find a CTA; 2, 3, 4, 5
+    const int n = threadIdx.x == 0 ? 1 : threadIdx.x == 1 ? max(1, fit) : threadIdx.x;             // whole; as many as find a CTA; 2, 3, 4; (the tail)
     sm_L[threadIdx.x] = max((sm_longest + n - 1) / n, min(4, max(sm_longest, 1)));
   }
   if (p.slots > 0) {
@@ -155,11 +160,22 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PagedPre
   if (threadIdx.x == 0) {
     float best = 3.0e38f;
     int cut = sm_L[0];
+    sm_tail = 0;
+    const int whole = n_items * p.heads, over = whole % ctas;        // the host keeps them inside 32 bits
+    const float share = (float)sm_total * p.heads / ctas, end = n_items > 0 ? 0.5f * ((float)sm_shortest + (float)sm_total / n_items) : 0.f;
     for (int k = 0; k < PLAN_CAND && p.slots > 0; ++k) {
+      if (k == PLAN_CAND - 1) {                                      // the tail
+        if (n_items > PLAN_TAIL || whole <= ctas || over == 0 || 2 * over > ctas) continue;
+        const int tail = (over + p.heads - 1) / p.heads, n = ctas / over;
+        const int64_t parts = (int64_t)tail * p.heads * n;
+        if (parts > p.slots || n_items + tail * (n - 1) > p.max_pieces) continue;
+        const float est = share + 0.5f * end / n + PLAN_COST * fmaxf(1.f, (float)parts / ctas);
+        if (est < best) { best = est; cut = sm_longest; sm_tail = tail; sm_tail_parts = n; }
+        continue;
+      }
       const int64_t n = (int64_t)sm_pieces[k] * p.heads, parts = (int64_t)sm_parts[k] * p.heads;
       if (k > 0 && (parts > p.slots || sm_pieces[k] > p.max_pieces)) continue;
-      const float share = (float)sm_total * p.heads / ctas;
-      const float est = (n <= ctas ? (float)sm_L[k] : share + 0.5f * sm_L[k]) + (parts > 0 ? PLAN_COST * fmaxf(1.f, (float)parts / ctas) : 0.f);
+      const float est = (n <= ctas ? (float)sm_L[k] : share + 0.5f * fminf(end, (float)sm_L[k])) + (parts > 0 ? PLAN_COST * fmaxf(1.f, (float)parts / ctas) : 0.f);
       if (est < best) { best = est; cut = sm_L[k]; }
     }
     sm_cut = max(cut, 1);
@@ -167,27 +183,49 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PagedPre
   __syncthreads();
   const unsigned L = sm_cut;
   auto bucket = [](int t) { return PLAN_BUCKETS - 1 - min(t, PLAN_BUCKETS - 1); };                  // longest first
-  // an item of t tiles goes in n pieces: t % n of them one tile longer than the others
-  items([&](const PlanItem& it) {
-    const int t = it.j1 - it.j0 + 1, n = max(1, (int)((t + L - 1) / L)), rem = t % n;
-    if (rem) atomicAdd(&hist[bucket(t / n + 1)], rem);
-    atomicAdd(&hist[bucket(t / n)], n - rem);
-  });
-  __syncthreads();
-  {                                                                  // exclusive prefix sums of the buckets, a thread each
+  // exclusive prefix sums of the buckets, a thread each -> the sum of all
+  auto prefix = [&]() {
+    __syncthreads();
     const int own = hist[threadIdx.x];
     int x = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
-    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane] : 0);
+    const int sum = warp_sums[lane], before = __reduce_add_sync(0xffffffffu, lane < warp ? sum : 0), all = __reduce_add_sync(0xffffffffu, sum);
     hist[threadIdx.x] = before + x - own;
-    if (threadIdx.x == PLAN_THREADS - 1) { p.head->n_pieces = min(before + x, p.max_pieces); p.head->queue = 0; }
+    __syncthreads();
+    return all;
+  };
+  // The tail's items: the shortest, of equally long ones the last (by place, not by the order of the list, which no two runs share: a cut item
+  // is rounded otherwise than a whole one).
+  const int tail = sm_tail;
+  if (tail > 0) {
+    if ((int)threadIdx.x < n_items) {
+      const PlanItem it = kept[threadIdx.x];
+      int in_front = 0;
+      for (int i = 0; i < n_items; ++i) {
+        const PlanItem& o = kept[i];
+        const int d = (o.j1 - o.j0) - (it.j1 - it.j0);
+        in_front += d > 0 || (d == 0 && (o.b < it.b || (o.b == it.b && o.i0 < it.i0)));
+      }
+      kept[threadIdx.x].cut = in_front >= n_items - tail;
+    }
+    __syncthreads();
   }
-  __syncthreads();
+  // an item of t tiles goes in n pieces: t % n of them one tile longer than the others
+  auto pieces_of = [&](const PlanItem& it, int t) {
+    return tail > 0 ? (it.cut ? max(1, min(sm_tail_parts, t)) : 1) : max(1, (int)((t + L - 1) / L));
+  };
   items([&](const PlanItem& it) {
-    const int t = it.j1 - it.j0 + 1, n = max(1, (int)((t + L - 1) / L)), rem = t % n, len = t / n;
+    const int t = it.j1 - it.j0 + 1, n = pieces_of(it, t), rem = t % n;
+    if (rem) atomicAdd(&hist[bucket(t / n + 1)], rem);
+    atomicAdd(&hist[bucket(t / n)], n - rem);
+  });
+  const int n_pieces = prefix();
+  if (threadIdx.x == 0) { p.head->n_pieces = min(n_pieces, p.max_pieces); p.head->queue = 0; }
+  items([&](const PlanItem& it) {
+    const int t = it.j1 - it.j0 + 1, n = pieces_of(it, t), rem = t % n, len = t / n;
     int slot = 0;
     if (n > 1) {
       slot = atomicAdd(&sm_slots, n * p.heads);
@@ -942,8 +980,8 @@ extern "C" int daisy_b200_paged_attend(const daisy_b200_pages* cache, const void
   // 17.5 us with it, 9.9 without
   const int64_t per_seq = (T + p.toks - 1) / p.toks, items = per_seq * cache->n_seq * p.heads;
   if (!cu && longest <= PP_SHORT) p.counted = (int)per_seq;
-  // Cutting pays where items are fewer than three a SM
-  if (tokens / p.toks * p.heads >= 3 * (int64_t)sms) p.slots = 0;
+  // Cutting pays where items are fewer than four a SM
+  if (tokens / p.toks * p.heads >= 4 * (int64_t)sms) p.slots = 0;
   cudaError_t e = cudaSuccess;
   if (!p.counted) e = daisy_host::launch_dependent(paged_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, p, sms);
   const dim3 grid((unsigned)(p.counted ? std::min<int64_t>(items, sms) : sms));
