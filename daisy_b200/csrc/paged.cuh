@@ -71,4 +71,7 @@ static inline int paged_cache(const daisy_b200_pages* c, int D, daisy::PagedCach
   return DAISY_OK;
 }
 
+// A window that holds every position that the table can is none: differences of positions and windows stay inside 32 bits.
+static inline int paged_window(const daisy_b200_pages* c, int window) { return window > 0 && window < (int64_t)c->width * c->page ? window : 0; }
+
 }  // namespace daisy_host

@@ -736,7 +736,7 @@ extern "C" int daisy_b200_paged_decode_step(const daisy_b200_pages* cache, const
   p.o_sb = o_sb; p.o_sh = o_sh;
   p.out = (__nv_bfloat16*)out;
   p.lens = lens; p.cos = cos; p.sin = sin; p.ve_gate = ve_gate_logit;
-  p.window = window; p.table_rows = table_rows;
+  p.window = daisy_host::paged_window(cache, window); p.table_rows = table_rows;
   p.qscale = scale * 1.4426950408889634f;
   p.eps = eps; p.flags = flags; p.status = status_word;
   const unsigned grid = (unsigned)(sms * pd_ctas(nq));
@@ -791,7 +791,7 @@ extern "C" int daisy_b200_paged_attend_few(const daisy_b200_pages* cache, const 
   if (pairs >= (int64_t)1 << 31 || blocks * pairs >= ((int64_t)1 << 31) - 65536) return DAISY_EUNSUPPORTED;
   p.q = (const __nv_bfloat16*)q; p.q_sb = q_sb; p.q_st = q_st; p.q_sh = q_sh;
   p.out = (__nv_bfloat16*)out; p.o_sb = o_sb; p.o_st = o_st; p.o_sh = o_sh;
-  p.lens = lens; p.window = window > 0 ? window : 0;
+  p.lens = lens; p.window = daisy_host::paged_window(cache, window);
   p.qscale = scale * 1.4426950408889634f;
   p.status = status_word;
   const unsigned grid = (unsigned)(sms * pd_ctas(PD_FEW));

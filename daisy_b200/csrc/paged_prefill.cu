@@ -944,7 +944,7 @@ extern "C" int daisy_b200_paged_attend(const daisy_b200_pages* cache, const void
   p.G = Hq / cache->H;
   p.lgp = prefill_lgp(p.G);
   p.heads = Hq >> p.lgp;
-  p.window = window > 0 ? window : 0;
+  p.window = daisy_host::paged_window(cache, window);
   int64_t longest = ((int64_t)cache->width * cache->page + PP_BN - 1) / PP_BN;
   if (p.window > 0) longest = std::min<int64_t>(longest, ((int64_t)p.window + (2 * PP_BM >> p.lgp)) / PP_BN + 2);
   p.toks = prefill_toks(sms, tokens, cache->n_seq, Hq, p.lgp, longest);

@@ -183,6 +183,8 @@ class PagedRunner:
         table = c.table.index_select(0, ints[:n])
         start, lens, cu = ints[n:2 * n], ints[2 * n:3 * n], ints[3 * n:]
         x = torch.cat(list(prompts))[None]
+        if ends[-1] == 0:
+            return list(x[0].split(counts))
         for i, a in enumerate(self.layers):
             x = a.prefill_paged(x, None, c, i, table, start, lens, self.window, cu)
         c.advance(slots, counts)

@@ -539,6 +539,25 @@ def test_attend_idle_and_refused_sequences(T):
     assert torch.isfinite(y.float()).all() and (y[0, 2 * T:] == 3.0).all()
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 40, 200])
+@pytest.mark.parametrize("T", [3, 150])
+@pytest.mark.parametrize("bounded", [True, False])
+def test_windows_longer_than_any_sequence_are_none(window, T, bounded):
+    from daisy_b200 import ops
+    H, page, lens = 2, 16, [160, 190]
+    pool = Pool(lens, [1, 1], H, page, torch.bfloat16, seed=155, extra_entries=0)
+    q = _norm(torch.randn(2, T, H, D, generator=_gen(156))).bfloat16().cuda()
+    x = [t.cuda() for t in _randn(_gen(157), 2, 1, 3 * H, D).split(H, 2)]
+    cos, sin = (t.cuda() for t in _tables(200))
+    got = []
+    for w in (window, None):
+        k_pages, v_pages, table = pool.gpu()
+        got.append((ops.paged_attend(q, k_pages, v_pages, table, _ints(lens), w, bounded_qk=bounded),
+                    ops.paged_decode_step(*x, k_pages, v_pages, table, _ints(lens), w, cos, sin, eps=EPS)))
+    _status()
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 def test_offsets_past_32_bits():
     """Pages whose element offsets need more than 32 bits."""
     from daisy_b200 import ops
@@ -670,6 +689,7 @@ def test_runner_serves_sequences_that_come_and_go(window, page, graph):
     slot = {}
     prompt(["a", "b"], [150, 3])
     steps(["a", "b"], 5)
+    assert [y.shape for y in runner.prefill([torch.zeros(0, dim, dtype=torch.bfloat16, device="cuda")] * 2, [0, 1])] == [(0, dim)] * 2
     prompt(["b"], [70])
     prompt(["c", "a"], [300, 4])
     steps(["a", "b", "c"], 40)
