@@ -5,8 +5,8 @@
 // share a key head: row r is query r / pack, head r % pack, so that a few queries of grouped heads fill the rows.  Tiles of 128 keys.
 // Long items of a call with few of them are cut along the keys into pieces, whose sums (fp32) a last launch joins in their
 // order.  The lengths are on the device, so a first, one-block launch works out the pieces, longest first, and the attention
-// kernel's CTAs draw them one by one.  Where all sequences have as many queries and nothing would be cut, the items are counted off
-// instead, in one launch.
+// kernel's CTAs draw them one by one.  Where nothing would be cut and the sequences have as many queries each, or are few, the items are
+// counted off instead, in one launch.
 //
 // Roles (as in the dense prefill kernel): two softmax warpgroups a stream, 64 key columns each, where the caller bounds the
 // logits (no running maximum is needed then), else one a stream with the whole row and a lazily refreshed reference maximum; a
@@ -43,7 +43,7 @@ struct PagedPrefillParams {
   const int *lens, *cu;
   int T, Hq, G, window, toks;        // toks: queries of an item, 256 or 128 rows / pack
   int lgp, heads;                    // pack = 1 << lgp; heads = Hq / pack
-  int counted;                       // > 0: items without a plan, so many a sequence
+  int counted;                       // > 0: items without a plan, so many a sequence (packed: as the offsets say, up to 32 sequences)
   float scale_log2;
   int* status;
   PlanHead* head;
@@ -318,6 +318,17 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     if (lane == 0) { prefetch_tmap(&tm_q); prefetch_tmap(&tm_k); prefetch_tmap(&tm_v); }
     // the plan's words come from L2: this grid was there before they were written
     int n_work = p.counted * p.c.n_seq * p.heads;                   // with a plan: known with the first piece
+    // packed sequences without a plan, a lane each: queries, and items up to it and including it
+    SeqQueries mine{0, 0, -1, false};
+    int upto = 0;
+    if (p.counted > 0 && p.cu) {
+      if (lane < p.c.n_seq) mine = seq_queries(p, lane);
+      if (mine.refused && p.status) p.status[0] = DAISY_EINVAL;
+      upto = (mine.n + p.toks - 1) / p.toks;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += y; }
+      n_work = __shfl_sync(0xffffffffu, upto, 31) * p.heads;
+    }
     const int ts = PP_BM >> p.lgp;                                  // queries of a stream
     const int lgr = min(p.c.lg, 7), boxes = PP_BN >> lgr;           // a tile is `boxes` boxes of 1 << lgr rows
     int n = 0;
@@ -354,7 +365,12 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       bool there = false;
       if (p.counted > 0) {                                           // a sequence's last queries first: they see most
         there = drawn < n_work;
-        if (there) {
+        if (there && p.cu) {
+          const int at = drawn / p.heads, b = __ffs(__ballot_sync(0xffffffffu, upto > at)) - 1;
+          const int n = __shfl_sync(0xffffffffu, mine.n, b), pos = __shfl_sync(0xffffffffu, mine.pos, b), row0 = __shfl_sync(0xffffffffu, mine.row0, b);
+          const int i0 = (__shfl_sync(0xffffffffu, upto, b) - 1 - at) * p.toks;
+          pc = Piece{b, i0, 0, 1 << 30, 0, 0, 1, pos < 0 ? -1 : pos + i0, min(p.toks, n - i0), row0 + i0, {0, 0}};
+        } else if (there) {
           const int at = drawn / p.heads, i = at / p.c.n_seq, i0 = (p.counted - 1 - i) * p.toks, b = at - i * p.c.n_seq;
           const SeqQueries sq = seq_queries(p, b);
           if (sq.refused && p.status && lane == 0) p.status[0] = DAISY_EINVAL;
@@ -976,10 +992,11 @@ extern "C" int daisy_b200_paged_attend(const daisy_b200_pages* cache, const void
   const bool f16 = (flags & DAISY_CACHE_FP16) != 0;
   // weights without a reference maximum reach 2^60, which float16 does not hold
   const bool bounded = (flags & DAISY_BOUNDED_QK) && !f16 && scale * 1.4426950408889634f * (float)D <= 60.f;
-  // No plan where all sequences have as many queries and tables, or windows, are too short for items of uneven length: 131 tokens x 6 heads
-  // 17.5 us with it, 9.9 without
-  const int64_t per_seq = (T + p.toks - 1) / p.toks, items = per_seq * cache->n_seq * p.heads;
-  if (!cu && longest <= PP_SHORT) p.counted = (int)per_seq;
+  // No plan where tables, or windows, are too short for items of uneven length, and the items can be counted off: as many for every sequence (131
+  // tokens x 6 heads 17.5 us with a plan, 9.9 without), or those of up to 32 in at most two items a SM (five of 20 to 200 tokens x 16 heads 18 and
+  // 10, of 90 to 900 31 and 21).  With more, the plan's order by length is worth its launch (nine of up to 1800 71 and 94)
+  const int64_t per_seq = (T + p.toks - 1) / p.toks, items = (cu ? tokens / p.toks + cache->n_seq : per_seq * cache->n_seq) * p.heads;
+  if (longest <= PP_SHORT && (!cu || (cache->n_seq <= 32 && items <= 2 * (int64_t)sms))) p.counted = cu ? 1 : (int)per_seq;
   // Cutting pays where items are fewer than four a SM
   if (tokens / p.toks * p.heads >= 4 * (int64_t)sms) p.slots = 0;
   cudaError_t e = cudaSuccess;

@@ -459,7 +459,7 @@ def _attend_case(prior, counts, Hq, H, page, window, dtype, seed, bounded=True, 
 
 
 @pytest.mark.parametrize("prior,counts", [([0], [1]), ([0], [127]), ([0], [129]), ([5], [300]), ([128], [128]), ([1, 500], [257, 257]), ([0, 130, 7, 64], [3, 200, 0, 90]),
-                                          ([700], [40]), ([255, 256, 257], [9, 9, 9])])
+                                          ([9] * 31 + [300], [11] * 31 + [140]), ([9] * 33, [5] * 32 + [30]), ([700], [40]), ([255, 256, 257], [9, 9, 9])])
 @pytest.mark.parametrize("window", [None, 1, 50, 128, 300])
 @pytest.mark.parametrize("dtype,bounded", [(torch.bfloat16, True), (torch.bfloat16, False), (torch.float16, True)])
 def test_attend(prior, counts, window, dtype, bounded):
