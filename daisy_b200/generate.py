@@ -239,6 +239,10 @@ class PagedRunner:
     @torch.inference_mode()
     def step_graph(self, x: torch.Tensor) -> torch.Tensor:
         """:meth:`step` from the recording; the result is a fixed buffer, overwritten by the next call."""
+        if self._graph is None:
+            raise RuntimeError("capture_step records the step first")
+        if x.shape != self._gx.shape:
+            raise ValueError(f"x must be {list(self._gx.shape)}, got {list(x.shape)}")
         slots = self._begin_step()
         self._gx.copy_(x)
         self._graph.replay()

@@ -607,7 +607,8 @@ int daisy_b200_paged_decode_step(const daisy_b200_pages* cache, const void* q_ne
 
 /* Attention of a chunk of every sequence, whose keys and values are in the pages already (daisy_b200_paged_append): query i of
  * the n of sequence b stands at position lens[b] - n + i and sees the keys of positions max(0, own - window + 1) .. own
- * (window <= 0: all up to its own).  For prompts behind a cached prefix, prompts in pieces, drafted tokens.
+ * (window <= 0: all up to its own).  For prompts behind a cached prefix, prompts in pieces, drafted tokens.  Rows that no query of the
+ * chunk sees may hold anything; an infinity or NaN in a value row that some of its queries see may reach the others.
  *   q          prepared (q_out of daisy_b200_paged_append), logical [B,T,Hq,D] with strides (s_b,s_t,s_h), of the PAGES' type;
  *              Hq a multiple of the cache's H
  *   lens       int32 [n_seq]: tokens of the sequence with this chunk, negative: idle

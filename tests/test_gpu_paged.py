@@ -653,6 +653,28 @@ def _stack(L, H, dim):
     return layers
 
 
+def test_runner_refusals():
+    from daisy_b200 import PagedRunner
+    dim = 2 * D
+    runner = PagedRunner(_stack(1, 2, dim), 50, pages=4, max_seqs=2, max_len=100, page=32)
+    x = torch.zeros(2, 1, dim, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError):                                # nothing recorded
+        runner.step_graph(x)
+    runner.capture_step(dim)
+    slot = runner.add()
+    for bad in (x[:1], x[0]):
+        with pytest.raises(ValueError):
+            runner.step_graph(bad)
+    with pytest.raises(RuntimeError):                                # a sequence is there
+        runner.capture_step(dim)
+    with pytest.raises(ValueError):
+        runner.prefill([x[0], x[1]], [slot, slot])
+    with pytest.raises(ValueError):                                  # more than the table holds
+        runner.prefill([torch.zeros(101, dim, dtype=torch.bfloat16, device="cuda")], [slot])
+    assert runner.cache.length == [0, -1] and len(runner.cache.book.free) == 4
+    _status()
+
+
 @pytest.mark.parametrize("window,page", [(None, 16), (90, 32), (33, 64)])
 @pytest.mark.parametrize("graph", [False, True])
 def test_runner_serves_sequences_that_come_and_go(window, page, graph):
