@@ -84,7 +84,7 @@ __device__ __forceinline__ int last_tile(int pos, int n) { return (pos + n - 1) 
 // where all pieces find a CTA, and PLAN_COST tiles' time for every piece of a cut item
 // (its sums are written, and read again by the last: 8192 tokens x 16 heads cut in halves 322 us, whole 278).  The last candidate cuts only
 // the shortest items, as many as whole rounds of all CTAs leave over, into as many pieces as find a CTA then (8192 queries x 16 heads over 65536
-// keys, 512 items: 3755 us whole, 3480 so).
+// keys, 512 items: 3700 us whole, 3400 so; three sequences of up to 1500 queries behind up to 9000, whose items' lengths make no rounds: 141 and 152).
 constexpr float PLAN_COST = 8.f;
 constexpr int PLAN_THREADS = 1024, PLAN_CAND = 6, PLAN_BUCKETS = 1024, PLAN_KEPT = 1024, PLAN_TAIL = 256;
 struct PlanItem { int b, i0, j0, j1, pos, n, row0, cut; };          // j1 < j0: queries that see nothing
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PagedPre
     const float share = (float)sm_total * p.heads / ctas, end = n_items > 0 ? 0.5f * ((float)sm_shortest + (float)sm_total / n_items) : 0.f;
     for (int k = 0; k < PLAN_CAND && p.slots > 0; ++k) {
       if (k == PLAN_CAND - 1) {                                      // the tail
-        if (n_items > PLAN_TAIL || whole <= ctas || over == 0 || 2 * over > ctas) continue;
+        if (n_items > PLAN_TAIL || whole <= ctas || over == 0 || 2 * over > ctas || sm_longest > 2 * sm_shortest) continue;
         const int tail = (over + p.heads - 1) / p.heads, n = ctas / over;
         const int64_t parts = (int64_t)tail * p.heads * n;
         if (parts > p.slots || n_items + tail * (n - 1) > p.max_pieces) continue;
@@ -352,11 +352,18 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       }
     };
     int drawn = blockIdx.x;                                         // the first one is this CTA's own number, later ones are drawn
+    int4 px = make_int4(0, 0, 0, 0), py = px, pz = px;              // its piece
+    auto fetch_piece = [&]() {
+      if (p.counted > 0 || drawn / p.heads >= p.max_pieces) return;
+      const int4* src = reinterpret_cast<const int4*>(p.pieces + drawn / p.heads);
+      px = __ldcg(src); py = __ldcg(src + 1); pz = __ldcg(src + 2);
+    };
     auto draw = [&]() {
       if (p.counted > 0) { drawn += gridDim.x; return; }
       int x = 0;
       if (lane == 0) x = atomicAdd(&p.head->queue, 1);
       drawn = (int)gridDim.x + __shfl_sync(0xffffffffu, x, 0);
+      fetch_piece();
     };
     auto publish = [&](int rd, PagedItem& g) {
       const int slot = rd % PP_NITEM;
@@ -377,11 +384,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           pc = Piece{b, i0, 0, 1 << 30, 0, 0, 1, sq.pos < 0 ? -1 : sq.pos + i0, min(p.toks, sq.n - i0), sq.row0 + i0, {0, 0}};
         }
       } else if (drawn / p.heads < p.max_pieces) {
-        const int4* src = reinterpret_cast<const int4*>(p.pieces + drawn / p.heads);
-        const int4 x = __ldcg(src), y = __ldcg(src + 1), z = __ldcg(src + 2);
         if (rd == 0) n_work = __ldcg(&p.head->n_pieces) * p.heads;
         there = drawn < n_work;
-        pc = Piece{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w, z.x, z.y, {0, 0}};
+        pc = Piece{px.x, px.y, px.z, px.w, py.x, py.y, py.z, py.w, pz.x, pz.y, {0, 0}};
       }
       if (there) {
         g.b = pc.b; g.h = drawn % p.heads;
@@ -410,9 +415,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         bars->item[slot] = g;
         mbar_arrive(&bars->i_full[slot]);
       }
-      if (g.b >= 0) draw();
     };
     PagedItem g, g_next;
+    fetch_piece();
     publish(0, g);
     if (ok && g.b >= 0) load_q(g);
     for (int rd = 0; ok && g.b >= 0; ++rd, g = g_next) {
@@ -426,14 +431,18 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       int from = 0, cur = 0, ahead = 0;
       if (g.jhi >= g.jlo) { from = (g.jlo * PP_BN) >> p.c.lg; cur = entries(from); ahead = entries(from + 32); }
       bool next_out = false;
+      // The next item is drawn two tiles before this one's last: what is drawn at the start goes to a CTA that may be the last to come to it (8192
+      // queries x 16 heads over 65536 keys 3700 -> 3400 us)
+      if (g.jhi < g.jlo) draw();
       for (int j = g.jlo; j <= g.jhi && ok; ++j) {
+        if (j == max(g.jlo, g.jhi - 2)) draw();
         // a lane a box (32 is a multiple of the boxes of a tile); only those that hold a row somebody sees
         const int k0 = j * PP_BN, e_lo = k0 >> p.c.lg;
         if (e_lo >= from + 32) { from += 32; cur = ahead; ahead = entries(from + 32); }
         int pg = __shfl_sync(0xffffffffu, cur, e_lo - from + (lane & (boxes - 1)));
         const int b_first = max(g.see0 - k0, 0) >> lgr, b_last = (min(g.end - k0, PP_BN) - 1) >> lgr;
-        const bool mine = lane >= b_first && lane <= b_last;
-        if (mine && (unsigned)pg >= (unsigned)p.c.n_pages) {
+        const bool issues = lane >= b_first && lane <= b_last;
+        if (issues && (unsigned)pg >= (unsigned)p.c.n_pages) {
           if (p.status) p.status[0] = DAISY_EINVAL;
           pg = 0;
         }
@@ -444,7 +453,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           if (!wait(&bars->kv_empty[stage], ((n / PP_NSTAGE) & 1) ^ 1, 1)) { ok = false; break; }
           if (lane == 0) mbar_expect_tx(&bars->kv_full[stage], bytes);
           __syncwarp();
-          if (mine) {
+          if (issues) {
             uint8_t* dst = kv_tiles + stage * PP_TILE + (lane << (lgr + 7));
             const CUtensorMap* tm = kv ? &tm_v : &tm_k;
             tma_load_4d(dst, tm, &bars->kv_full[stage], 0, in_page, hk, pg);
