@@ -82,20 +82,21 @@ __device__ __forceinline__ int last_tile(int pos, int n) { return (pos + n - 1) 
 // How far items are cut: into pieces of at most L tiles, L from a few candidates by the estimate
 // total / CTAs + half a piece such as come last (they go longest first: halfway between the shortest item and the mean), or a longest piece
 // where all pieces find a CTA, and PLAN_COST tiles' time for every piece of a cut item
-// (its sums are written, and read again by the last: 8192 tokens x 16 heads cut in halves 322 us, whole 278).  The last candidate cuts only
+// (its sums are written, and read again by the last: 8192 tokens x 16 heads cut in halves 266 us, whole 233).  Whole items take no less than k of
+// the (k - 1) CTAs + 1st longest: of so many, one CTA has k.  The last candidate cuts only
 // the shortest items, as many as whole rounds of all CTAs leave over, into as many pieces as find a CTA then (8192 queries x 16 heads over 65536
-// keys, 512 items: 3700 us whole, 3400 so; three sequences of up to 1500 queries behind up to 9000, whose items' lengths make no rounds: 141 and 152).
-constexpr float PLAN_COST = 8.f;
+// keys, 512 items: 3700 us whole, 3400 so; three sequences of up to 1500 queries behind up to 9000, whose items make no rounds: 141 and 152).
+constexpr float PLAN_COST = 6.f;
 constexpr int PLAN_THREADS = 1024, PLAN_CAND = 6, PLAN_BUCKETS = 1024, PLAN_KEPT = 1024, PLAN_TAIL = 256;
 struct PlanItem { int b, i0, j0, j1, pos, n, row0, cut; };          // j1 < j0: queries that see nothing
 __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PagedPrefillParams p, int ctas) {
   __shared__ PlanItem kept[PLAN_KEPT];
   __shared__ int hist[PLAN_BUCKETS];
   __shared__ unsigned long long sm_total;
-  __shared__ int sm_longest, sm_shortest, sm_items, sm_slots, sm_cuts, sm_cut, sm_pieces[PLAN_CAND], sm_parts[PLAN_CAND], sm_L[PLAN_CAND], sm_tail, sm_tail_parts, warp_sums[32];
+  __shared__ int sm_longest, sm_shortest, sm_items, sm_slots, sm_cuts, sm_cut, sm_rounds, sm_full_rounds, sm_pieces[PLAN_CAND], sm_parts[PLAN_CAND], sm_L[PLAN_CAND], sm_tail, sm_tail_parts, warp_sums[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   hist[threadIdx.x] = 0;
-  if (threadIdx.x == 0) { sm_total = 0; sm_longest = 0; sm_shortest = 1 << 30; sm_items = 0; sm_slots = 0; sm_cuts = 0; }
+  if (threadIdx.x == 0) { sm_total = 0; sm_longest = 0; sm_shortest = 1 << 30; sm_items = 0; sm_slots = 0; sm_cuts = 0; sm_rounds = 0; sm_full_rounds = 0; }
   if (threadIdx.x < PLAN_CAND) { sm_pieces[threadIdx.x] = 0; sm_parts[threadIdx.x] = 0; }
   grid_dep_launch();
   grid_dep_wait();
@@ -138,6 +139,21 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PagedPre
     const int n = threadIdx.x == 0 ? 1 : threadIdx.x == 1 ? max(1, fit) : threadIdx.x;             // whole; as many as find a CTA; 2, 3, 4; (the tail)
     sm_L[threadIdx.x] = max((sm_longest + n - 1) / n, min(4, max(sm_longest, 1)));
   }
+  // Longer items than a kept one's, of equally long ones those in front (by place, not by the order of the list, which no two runs share: a
+  // cut item is rounded otherwise than a whole one).
+  int in_front = 0;
+  if (p.slots > 0 && n_items <= PLAN_TAIL && n_items * p.heads > ctas && (int)threadIdx.x < n_items) {
+    const PlanItem it = kept[threadIdx.x];
+    for (int i = 0; i < n_items; ++i) {
+      const PlanItem& o = kept[i];
+      const int d = (o.j1 - o.j0) - (it.j1 - it.j0);
+      in_front += d > 0 || (d == 0 && (o.b < it.b || (o.b == it.b && o.i0 < it.i0)));
+    }
+    for (int k = (in_front * p.heads + ctas - 1) / ctas; k * ctas < (in_front + 1) * p.heads; ++k) {
+      atomicMax(&sm_rounds, (k + 1) * (it.j1 - it.j0 + 1));
+      if ((k + 1) * ctas <= n_items * p.heads) atomicMax(&sm_full_rounds, (k + 1) * (it.j1 - it.j0 + 1));       // without the tail
+    }
+  }
   if (p.slots > 0) {
     __syncthreads();
     int pieces[PLAN_CAND] = {}, parts[PLAN_CAND] = {};
@@ -169,13 +185,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PagedPre
         const int tail = (over + p.heads - 1) / p.heads, n = ctas / over;
         const int64_t parts = (int64_t)tail * p.heads * n;
         if (parts > p.slots || n_items + tail * (n - 1) > p.max_pieces) continue;
-        const float est = share + 0.5f * end / n + PLAN_COST * fmaxf(1.f, (float)parts / ctas);
+        const float est = fmaxf(share + 0.5f * end / n, (float)sm_full_rounds) + PLAN_COST * fmaxf(1.f, (float)parts / ctas);
         if (est < best) { best = est; cut = sm_longest; sm_tail = tail; sm_tail_parts = n; }
         continue;
       }
       const int64_t n = (int64_t)sm_pieces[k] * p.heads, parts = (int64_t)sm_parts[k] * p.heads;
       if (k > 0 && (parts > p.slots || sm_pieces[k] > p.max_pieces)) continue;
-      const float est = (n <= ctas ? (float)sm_L[k] : share + 0.5f * fminf(end, (float)sm_L[k])) + (parts > 0 ? PLAN_COST * fmaxf(1.f, (float)parts / ctas) : 0.f);
+      const float est = (n <= ctas ? (float)sm_L[k] : fmaxf(share + 0.5f * fminf(end, (float)sm_L[k]), parts > 0 ? 0.f : (float)sm_rounds)) +
+                        (parts > 0 ? PLAN_COST * fmaxf(1.f, (float)parts / ctas) : 0.f);
       if (est < best) { best = est; cut = sm_L[k]; }
     }
     sm_cut = max(cut, 1);
@@ -197,20 +214,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) paged_plan_kernel(const PagedPre
     __syncthreads();
     return all;
   };
-  // The tail's items: the shortest, of equally long ones the last (by place, not by the order of the list, which no two runs share: a cut item
-  // is rounded otherwise than a whole one).
-  const int tail = sm_tail;
+  const int tail = sm_tail;                                          // the shortest items, of equally long ones the last
   if (tail > 0) {
-    if ((int)threadIdx.x < n_items) {
-      const PlanItem it = kept[threadIdx.x];
-      int in_front = 0;
-      for (int i = 0; i < n_items; ++i) {
-        const PlanItem& o = kept[i];
-        const int d = (o.j1 - o.j0) - (it.j1 - it.j0);
-        in_front += d > 0 || (d == 0 && (o.b < it.b || (o.b == it.b && o.i0 < it.i0)));
-      }
-      kept[threadIdx.x].cut = in_front >= n_items - tail;
-    }
+    if ((int)threadIdx.x < n_items) kept[threadIdx.x].cut = in_front >= n_items - tail;
     __syncthreads();
   }
   // an item of t tiles goes in n pieces: t % n of them one tile longer than the others
