@@ -140,7 +140,8 @@ def _same_bits(a, b):
 # ---------------------------------------------------------------------------------------------- append
 @pytest.mark.parametrize("starts,counts,Hq,H,page", [
     ([0], [1], 2, 2, 16), ([5], [1], 6, 3, 64), ([15, 16, 17], [1, 1, 1], 3, 3, 16), ([0, 7, 100], [40, 40, 40], 4, 1, 32),
-    ([3, 0, 250, 31, 9], [0, 70, 5, 0, 1], 4, 2, 64), ([0, 600], [257, 300], 8, 8, 128), ([0, 1000, 3], [33, 1, 600], 2, 2, 256)])
+    ([3, 0, 250, 31, 9], [0, 70, 5, 0, 1], 4, 2, 64), ([0, 600], [257, 300], 8, 8, 128), ([0, 1000, 3], [33, 1, 600], 2, 2, 256),
+    ([9 * b % 40 for b in range(40)], [5 * b % 7 for b in range(40)], 2, 1, 16), ([13 * b % 60 for b in range(1500)], [7 * b % 4 for b in range(1500)], 1, 1, 16)])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("strided", [False, True])
 def test_append(starts, counts, Hq, H, page, dtype, strided):
@@ -496,6 +497,37 @@ def test_attend_long_contexts_are_cut(prior, counts, Hq, H, window, dtype, bound
     """Few items with long contexts go in pieces: joined in a fixed order, the same bits every time."""
     a = _attend_case(prior, counts, Hq, H, 64, window, dtype, seed=131, bounded=bounded)
     assert torch.equal(a, _attend_case(prior, counts, Hq, H, 64, window, dtype, seed=131, bounded=bounded))
+
+
+@pytest.mark.parametrize("counts", [[7 * b % 12 for b in range(1300)], [9] * 1100])
+@pytest.mark.parametrize("longest", [200, 2500])
+@pytest.mark.parametrize("bounded", [True, False])
+def test_attend_many_sequences(counts, longest, bounded):
+    """More sequences than a warp counts, more items than the plan keeps; with and without a table long enough for a plan."""
+    prior = [31 * b % 40 for b in range(len(counts))]
+    prior[700] = longest
+    _attend_case(prior, counts, 1, 1, 16, None, torch.bfloat16, seed=136, bounded=bounded)
+
+
+@pytest.mark.parametrize("T", [2400, 2560, 2720])
+@pytest.mark.parametrize("dtype,bounded", [(torch.bfloat16, True), (torch.bfloat16, False), (torch.float16, False)])
+def test_attend_items_left_over_by_whole_rounds(T, dtype, bounded):
+    """150 to 170 items of like length: a few more than there are SMs, so that the last ones are cut."""
+    from daisy_b200 import ops
+    Hq, page, prior, window = 16, 64, 2300, 2000
+    pool = Pool([prior + T], [0], 1, page, dtype, seed=137)
+    q = torch.randn(1, T, Hq, D, generator=_gen(138))
+    q = (q / q.square().mean(-1, keepdim=True).sqrt()).to(dtype)
+    k_pages, v_pages, table = pool.gpu()
+    y = ops.paged_attend(q.cuda(), k_pages, v_pages, table, _ints([prior + T]), window, bounded_qk=bounded)
+    assert torch.equal(y, ops.paged_attend(q.cuda(), k_pages, v_pages, table, _ints([prior + T]), window, bounded_qk=bounded))
+    _status()
+    k, v = pool.rows(pool.k, 0, 0, prior + T), pool.rows(pool.v, 0, 0, prior + T)
+    for at in [*range(0, T, 300), T - 200, T - 90, T - 10]:          # ten queries here and there
+        own = prior + torch.arange(at, at + 10)
+        gap = own[:, None] - torch.arange(prior + T)[None]
+        ref, A, mass = _attention(q[0, at:at + 10].double(), k, v, (gap >= 0) & (gap < window))
+        _check(y[0, at:at + 10], ref, _attend_tol(ref, A, mass, window, dtype, v.abs().max(), bounded), f"queries from {at}")
 
 
 @pytest.mark.parametrize("few", [False, True])
