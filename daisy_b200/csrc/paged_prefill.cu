@@ -506,23 +506,24 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           const uint32_t s_tmem = tmem_base + s * 128, o_tmem = tmem_base + 256 + s * 128;
           if (j - 1 >= g.jlo_s[s] && j - 1 <= g.jhi_s[s]) {          // O_s += P_s(j-1) V_{j-1}
             const int n = n_base + 2 * (j - 1 - g.jlo) + 1, stage = n % PP_NSTAGE;
-            if (!wait(&bars->p_full[s], n_pv[s] & 1, 2)) { ok = false; break; }
-            ++n_pv[s];
             const bool v_seen = s == 1 && g.valid[0] && j - 1 >= g.jlo_s[0] && j - 1 <= g.jhi_s[0];
-            if (!v_seen) {
+            if (!v_seen) {                                           // V is there before the weights: what is to be cleared is cleared under the softmax
               if (!wait(&bars->kv_full[stage], (n / PP_NSTAGE) & 1, 3)) { ok = false; break; }
               const int k0 = (j - 1) * PP_BN, lo = max(g.see0 - k0, 0), hi = min(g.end - k0, PP_BN);
               if (lo > 0 || hi < PP_BN) {                            // rows that nobody sees
                 uint8_t* tile = kv_tiles + stage * PP_TILE + (lane & 7) * 16;
-                for (int r = lane >> 3; r < PP_BN; r += 4)
-                  if (r < lo || r >= hi) {
-                    *reinterpret_cast<uint4*>(tile + r * 128) = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(tile + PP_HALF + r * 128) = make_uint4(0, 0, 0, 0);
-                  }
+                auto clear = [&](int r) {
+                  *reinterpret_cast<uint4*>(tile + r * 128) = make_uint4(0, 0, 0, 0);
+                  *reinterpret_cast<uint4*>(tile + PP_HALF + r * 128) = make_uint4(0, 0, 0, 0);
+                };
+                for (int r = lane >> 3; r < lo; r += 4) clear(r);
+                for (int r = hi + (lane >> 3); r < PP_BN; r += 4) clear(r);
                 fence_proxy_async();
                 __syncwarp();
               }
             }
+            if (!wait(&bars->p_full[s], n_pv[s] & 1, 2)) { ok = false; break; }
+            ++n_pv[s];
             tc_fence_after();
             const uint32_t v_lo = v_lo0 + stage * (PP_TILE >> 4);
             umma_ts_lh_p(leader, o_tmem, s_tmem, v_lo, v_hi, idesc_pv, j - 1 == g.jlo_s[s] ? 0u : 1u);
