@@ -274,7 +274,7 @@ static_assert(sizeof(PagedBarriers) <= PP_BARS, "room for the barriers");
 template <int NSPLIT, bool F16>
 __global__ void __launch_bounds__(32 * (8 * NSPLIT + 2), 1)
 paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                     const __grid_constant__ CUtensorMap tm_v, const PagedPrefillParams p) {
+                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o, const PagedPrefillParams p) {
   static_assert(!(F16 && NSPLIT == 2), "weights without a reference maximum do not fit float16");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -321,7 +321,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 
   if (warp == TMA_WARP) {
     // ------------------------------------------------------------------ TMA producer: the warp as one, lane 0 issues
-    if (lane == 0) { prefetch_tmap(&tm_q); prefetch_tmap(&tm_k); prefetch_tmap(&tm_v); }
+    if (lane == 0) { prefetch_tmap(&tm_q); prefetch_tmap(&tm_k); prefetch_tmap(&tm_v); prefetch_tmap(&tm_o); }
     // the plan's words come from L2: this grid was there before they were written
     int n_work = p.counted * p.c.n_seq * p.heads;                   // with a plan: known with the first piece
     // packed sequences without a plan, a lane each: queries, and items up to it and including it
@@ -604,8 +604,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       if (g->parts > 1) leave(g, zero, PP_NEG, 0.f);
       else store_row(g, none);
     };
-    // the last step of an item: l, m of this lane's row, sums in O.  box: 32 rows of 128 bytes (two with NSPLIT = 1) of the item's Q buffer,
-    // which its last scores have left, turn the lanes' rows into whole row segments
+    // the last step of an item: l, m of this lane's row, sums in O.  They leave through the item's Q buffer, which its last scores have left: a bulk
+    // copy of a warp's 32 rows (read back and stored by rows 8192 queries x 16 heads took 233 us, window 512 61; so 227 and 57.5)
     auto finish = [&](const PagedItem* g, float m, float l, uint8_t* box) {
       uint32_t o[COLS];
 #pragma unroll
@@ -613,6 +613,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       tc_wait_ld();
       if (g->parts > 1) {
         leave(g, o, m, l);
+        fence_proxy_async();                                         // the Q buffer, which held the row sums, is next written by a copy
       } else {
         const float inv = 1.0f / l;
         const int n_rows = (g->n[s] << p.lgp) - quarter * 32;
@@ -626,26 +627,46 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(o[hc * 64 + 8 * c + e]) * inv;
             *reinterpret_cast<uint4*>(mine + row * 128 + ((c ^ (row & 7)) << 4)) = pack8(y);
           }
-          __syncwarp();
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (n_rows >= 32) {
+          if (lane == 0) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + (lane >> 3);
-            const uint4 v = *reinterpret_cast<const uint4*>(mine + (quarter * 32 + r) * 128 + (((lane & 7) ^ (r & 7)) << 4));
-            if (r < n_rows) *reinterpret_cast<uint4*>(row_at(g, quarter * 32 + r) + half * 64 + (lane & 7) * 8 + hc * 64) = v;
+            for (int hc = 0; hc < COLS / 64; ++hc)
+              tma_store_4d(&tm_o, box + hc * PP_HALF + quarter * 4096, half * 64 + hc * 64, g->h << p.lgp, g->row0 + s * ts + quarter * (32 >> p.lgp), g->bq);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
+        } else {                                                     // the end of a sequence: the rows behind it are another's
+#pragma unroll
+          for (int hc = 0; hc < COLS / 64; ++hc)
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) {
+              const int r = i * 4 + (lane >> 3);
+              if (r >= n_rows) break;
+              *reinterpret_cast<uint4*>(row_at(g, quarter * 32 + r) + half * 64 + (lane & 7) * 8 + hc * 64) =
+                  *reinterpret_cast<const uint4*>(box + hc * PP_HALF + (quarter * 32 + r) * 128 + (((lane & 7) ^ (r & 7)) << 4));
+            }
+          fence_proxy_async();                                       // as above
         }
       }
       // the next item's first product into O_s follows this warp's next weights, which follow these loads
       tc_fence_before();
-      fence_proxy_async();                                           // the Q buffer is next written by a copy
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->q_empty[s][n_o % PP_NQBUF]);
       ++n_o;
+    };
+    // The item before has left its Q buffer: asked when the next one begins, two items before that buffer is wanted
+    auto buffer_free = [&]() {
+      __syncwarp();
+      if (lane == 0 && n_o > 0) {
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        mbar_arrive(&bars->q_empty[s][(n_o - 1) % PP_NQBUF]);
+      }
     };
 
     for (int rd = 0; ok && (item = next_item(rd)); item_done(rd), ++rd) {
       const int q0 = item->q0[s], jlo = item->jlo_s[s], jhi = item->jhi_s[s];
       if (jhi < jlo) { without_tiles(item); continue; }
+      buffer_free();
       const int q_row = q0 + (row >> p.lgp);
       uint8_t* q_buf = q_tiles + ((n_o % PP_NQBUF) * 2 + s) * PP_TILE;
       auto scores_there = [&]() -> bool {
@@ -825,6 +846,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         finish(item, m_ref, l, q_buf);
       }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   // ------------------------------------------------------------------ teardown
@@ -968,8 +990,8 @@ extern "C" int daisy_b200_paged_attend(const daisy_b200_pages* cache, const void
   if (!daisy_aligned16(q) || !daisy_aligned16(out) || ((q_sb | q_st | q_sh | o_sb | o_st | o_sh) & 7) || (reinterpret_cast<uintptr_t>(lens) & 3) ||
       (reinterpret_cast<uintptr_t>(cu) & 3) || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return DAISY_EALIGN;
-  // a zero stride on a dimension longer than 1 is a broadcast view, which the tile loads cannot express
-  if ((T > 1 && q_st <= 0) || (Hq > 1 && q_sh <= 0) || (B > 1 && q_sb <= 0)) return DAISY_EINVAL;
+  // a zero stride on a dimension longer than 1 is a broadcast view, which the tile copies cannot express
+  if ((T > 1 && (q_st <= 0 || o_st <= 0)) || (Hq > 1 && (q_sh <= 0 || o_sh <= 0)) || (B > 1 && (q_sb <= 0 || o_sb <= 0))) return DAISY_EINVAL;
   const int sms = daisy_host::sm_count_cached();
   if (sms <= 0) return DAISY_ENODEV;
   const int64_t tokens = (int64_t)B * T;
@@ -984,11 +1006,12 @@ extern "C" int daisy_b200_paged_attend(const daisy_b200_pages* cache, const void
   if (workspace_bytes < room.end) return DAISY_EWORKSPACE;
   if ((room.max_pieces + 1) * Hq >= ((int64_t)1 << 31) - 4096) return DAISY_EUNSUPPORTED;
   if (const int rc = paged_prefill_smem(); rc != DAISY_OK) { (void)cudaGetLastError(); return rc; }
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to;
   auto sb = [](int64_t s, int64_t n) { return (uint64_t)(n == 1 ? 16 : s * 2); };
   int rc;
   const uint32_t box = (uint32_t)(cache->page < PP_BN ? cache->page : PP_BN);
   if ((rc = make_tmap_packed_rows(&tq, q, D, Hq, T, B, sb(q_sh, Hq), sb(q_st, T), sb(q_sb, B), 1u << p.lgp, (uint32_t)(PP_BM >> p.lgp))) != DAISY_OK) return rc;
+  if ((rc = make_tmap_packed_rows(&to, out, D, Hq, T, B, sb(o_sh, Hq), sb(o_st, T), sb(o_sb, B), 1u << p.lgp, 32u >> p.lgp)) != DAISY_OK) return rc;       // a warp's rows
   if ((rc = daisy_host::make_tmap_bf16_dthb(&tk, cache->k, D, cache->page, cache->H, cache->n_pages, cache->p_sr * 2, sb(cache->p_sh, cache->H),
                                             sb(cache->p_sb, cache->n_pages), 64, box)) != DAISY_OK) return rc;
   if ((rc = daisy_host::make_tmap_bf16_dthb(&tv, cache->v, D, cache->page, cache->H, cache->n_pages, cache->p_sr * 2, sb(cache->p_sh, cache->H),
@@ -1019,9 +1042,9 @@ extern "C" int daisy_b200_paged_attend(const daisy_b200_pages* cache, const void
   if (!p.counted) e = daisy_host::launch_dependent(paged_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, p, sms);
   const dim3 grid((unsigned)(p.counted ? std::min<int64_t>(items, sms) : sms));
   if (e == cudaSuccess) {
-    if (bounded)  e = daisy_host::launch_dependent(paged_prefill_kernel<2, false>, grid, dim3(576), PP_SMEM, st, tq, tk, tv, p);
-    else if (f16) e = daisy_host::launch_dependent(paged_prefill_kernel<1, true>, grid, dim3(320), PP_SMEM, st, tq, tk, tv, p);
-    else          e = daisy_host::launch_dependent(paged_prefill_kernel<1, false>, grid, dim3(320), PP_SMEM, st, tq, tk, tv, p);
+    if (bounded)  e = daisy_host::launch_dependent(paged_prefill_kernel<2, false>, grid, dim3(576), PP_SMEM, st, tq, tk, tv, to, p);
+    else if (f16) e = daisy_host::launch_dependent(paged_prefill_kernel<1, true>, grid, dim3(320), PP_SMEM, st, tq, tk, tv, to, p);
+    else          e = daisy_host::launch_dependent(paged_prefill_kernel<1, false>, grid, dim3(320), PP_SMEM, st, tq, tk, tv, to, p);
   }
   if (e == cudaSuccess && !p.counted && p.slots > 0)
     e = bounded ? daisy_host::launch_dependent(paged_join_kernel<2>, dim3(sms * 4), dim3(256), 0, st, p) : daisy_host::launch_dependent(paged_join_kernel<1>, dim3(sms * 4), dim3(256), 0, st, p);
