@@ -961,7 +961,7 @@ static int prefill_lgp(int G) {
   return l;
 }
 // Queries of an item: 256 rows, or 128 where all items of that size find an SM and no item is long (`longest`: key tiles that the table or
-// the window leaves).  A tile takes one stream as long as two (1.57 us), so that the second one costs only where it adds tiles: 128 queries of
+// the window leaves).  A tile takes one stream as long as two (1.7 us), so that the second one costs only where it adds tiles: 128 queries of
 // 8 heads over one key head and 131000 keys 102 us with items of 128 rows, 69 with 256.
 constexpr int64_t PP_SHORT = 16;
 static int prefill_toks(int sms, int64_t tokens, int n_seq, int Hq, int lgp, int64_t longest) {
