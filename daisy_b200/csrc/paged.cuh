@@ -23,6 +23,12 @@ __device__ __forceinline__ uint4 pack8_16(const float* f) {
   return make_uint4(pack16<F16>(f[0], f[1]), pack16<F16>(f[2], f[3]), pack16<F16>(f[4], f[5]), pack16<F16>(f[6], f[7]));
 }
 
+// Softmax weights are powers of two over a reference that lies this far under the row's maximum: float16 has a floor of 2^-25 and room up to 2^15,
+// bf16 neither.  With the references' lag of up to 2^8 a float16 weight reaches 2^15, and is off by at most 2^-32 of the largest one
+// beside its rounding (with a reference at the maximum 2^-25: 4096 rows at 2^-25.3 behind one at 1 were not seen at all).
+template <bool F16>
+constexpr float WEIGHT_ROOM = F16 ? 7.f : 0.f;
+
 struct PagedCache {
   char *k, *v;                       // pages [n_pages, H, page, 128] of 16-bit values
   int64_t p_sb, p_sh, p_sr;          // element strides of page, head, row

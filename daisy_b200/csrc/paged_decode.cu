@@ -11,7 +11,8 @@
 // A warp takes a tile straight from memory into the operands of mma.m16n8k16 (keys or channels are the 16, query heads the 8; every lane
 // loads whole 16-byte pieces, the order of channels in a product is free): scores S^T = K Q^T, then O^T += V^T P^T.  On CUDA cores
 // the same work is 22 instructions for 16 bytes and lane, a third of the SM's issue slots for one query head and over all of them for
-// four.  Queries and weights go in as sums of two 16-bit values (two products each): scores and weights keep 16 bits and more.
+// four.  Queries and weights go in as sums of two 16-bit values (two products each): scores and weights keep 16 bits and more, weights of float16
+// pages down to 2^-16 of the largest, below that 2^-32 of it (WEIGHT_ROOM).
 #include "paged.cuh"
 
 //
@@ -515,13 +516,13 @@ __global__ void __launch_bounds__(32 * PD_WARPS, pd_ctas(8 * NT)) paged_decode_k
       for (int n = 0; n < NT; ++n) {
         float t0 = fmaxf(s[n][0], s[n][2]), t1 = fmaxf(s[n][1], s[n][3]);
         // the reference follows the maximum only when that has grown by over 2^8: sums stay far inside their range
-        if (__any_sync(0xffffffffu, t0 > m[n][0] + 8.f || t1 > m[n][1] + 8.f)) {
+        if (__any_sync(0xffffffffu, t0 > m[n][0] + (8.f + WEIGHT_ROOM<F16>) || t1 > m[n][1] + (8.f + WEIGHT_ROOM<F16>))) {
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
             t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
             t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
           }
-          t0 = fmaxf(t0, m[n][0]); t1 = fmaxf(t1, m[n][1]);
+          t0 = fmaxf(t0 - WEIGHT_ROOM<F16>, m[n][0]); t1 = fmaxf(t1 - WEIGHT_ROOM<F16>, m[n][1]);
           const float a0 = fast_exp2(m[n][0] - t0), a1 = fast_exp2(m[n][1] - t1);
           m[n][0] = t0; m[n][1] = t1;
           l[n][0] *= a0; l[n][1] *= a1;

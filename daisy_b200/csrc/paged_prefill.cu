@@ -789,7 +789,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             for (int i = 0; i < 128; ++i)
               if (!(i > lo && i <= hi)) r[i] = 0xff800000u;          // -inf
           }
-          // the reference maximum follows the row's only when that has grown by more than 8: weights stay below 2^8
+          // the reference follows the row's maximum only when that has grown by more than 8: weights stay below 2^8 (float16: 2^15, WEIGHT_ROOM)
           float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
@@ -798,7 +798,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             m2 = fmax3(m2, __uint_as_float(r[64 + i]), __uint_as_float(r[65 + i]));
             m3 = fmax3(m3, __uint_as_float(r[96 + i]), __uint_as_float(r[97 + i]));
           }
-          const float m_tgt = fmaxf(m_ref, fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * c2);
+          const float m_tgt = fmaxf(m_ref, fmaf(fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)), c2, -WEIGHT_ROOM<F16>));
           if (j == jlo) {
             m_ref = m_tgt;
           } else if (__any_sync(0xffffffffu, m_tgt - m_ref > 8.0f)) {
