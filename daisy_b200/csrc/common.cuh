@@ -40,10 +40,12 @@ __device__ __forceinline__ float fast_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// streaming 16-byte load that does not allocate in L1
+// Streaming 16-byte load that does not allocate in L1.  Coherent, like every load here: the non-coherent path (.nc, or the read-only
+// intrinsic) is defined for memory that nobody writes while the kernel lives, and a dependent grid (below) lives while the grids in front
+// of it still write what it will read.
 __device__ __forceinline__ uint4 ld_stream16(const void* p) {
   uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
   return r;
 }

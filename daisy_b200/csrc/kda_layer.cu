@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(SC_THREADS) kda_short_conv_kernel(const __grid
   }
   if (VARLEN && threadIdx.x <= SC_ROWS) {
     const int t = tblk + threadIdx.x;
-    toks[threadIdx.x] = t < p.T ? __ldg(p.tok + t) : make_int2(t, 0);
+    toks[threadIdx.x] = t < p.T ? p.tok[t] : make_int2(t, 0);
   }
 
   const int cg = threadIdx.x % (SC_COLS / SC_CH), slice = threadIdx.x / (SC_COLS / SC_CH);
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(SC_THREADS) kda_short_conv_kernel(const __grid
 #pragma unroll
       for (int h = 0; h < 2; ++h) {                                // 4 channels x 4 taps = 32 contiguous bytes
         float f[8];
-        unpack8(__ldg(reinterpret_cast<const uint4*>(p.w + (long long)c0 * 4 + h * 8)), f);
+        unpack8(*reinterpret_cast<const uint4*>(p.w + (long long)c0 * 4 + h * 8), f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) wt[h * 2 + i / 4][i % 4] = f[i];
       }
@@ -265,8 +265,8 @@ __global__ void __launch_bounds__(256) kda_out_norm_kernel(const OutNormParams p
   if (p.gbias) {                                                   // the bias of the gate's projection, as its Linear adds it
     const __nv_bfloat16* bsrc = p.gbias + (row % p.H) * ON_D + 8 * sub;
     float b1[8], b2[8];
-    unpack8(__ldg(reinterpret_cast<const uint4*>(bsrc)), b1);
-    unpack8(__ldg(reinterpret_cast<const uint4*>(bsrc + 64)), b2);
+    unpack8(*reinterpret_cast<const uint4*>(bsrc), b1);
+    unpack8(*reinterpret_cast<const uint4*>(bsrc + 64), b2);
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       const uint32_t r1 = pack_bf16(g1[e] + b1[e], g1[e + 1] + b1[e + 1]), r2 = pack_bf16(g2[e] + b2[e], g2[e + 1] + b2[e + 1]);
@@ -282,8 +282,8 @@ __global__ void __launch_bounds__(256) kda_out_norm_kernel(const OutNormParams p
   const float rstd = rsqrtf(ss * (1.0f / ON_D) + p.eps);
   if (p.w) {
     float w1[8], w2[8];
-    unpack8(__ldg(reinterpret_cast<const uint4*>(p.w + 8 * sub)), w1);
-    unpack8(__ldg(reinterpret_cast<const uint4*>(p.w + 64 + 8 * sub)), w2);
+    unpack8(*reinterpret_cast<const uint4*>(p.w + 8 * sub), w1);
+    unpack8(*reinterpret_cast<const uint4*>(p.w + 64 + 8 * sub), w2);
 #pragma unroll
     for (int e = 0; e < 8; ++e) { x1[e] *= rstd * w1[e]; x2[e] *= rstd * w2[e]; }
   } else {
@@ -341,8 +341,8 @@ __global__ void __launch_bounds__(256) kda_pack_rows_kernel(const uint4* x, cons
   grid_dep_wait();
   if (i >= n) return;
   const int64_t r = i / n8;
-  const int2 s = __ldg(tok + r);                       // its sequence's first token, its sequence
-  y[i] = __ldg(x + ((int64_t)s.y * T + idx[(int64_t)s.y * T + (r - s.x)]) * n8 + (i - r * n8));
+  const int2 s = tok[r];                       // its sequence's first token, its sequence
+  y[i] = x[((int64_t)s.y * T + idx[(int64_t)s.y * T + (r - s.x)]) * n8 + (i - r * n8)];
 }
 __global__ void __launch_bounds__(256) kda_unpack_rows_kernel(const uint4* y, const int* rank, const int* cu, uint4* out, int64_t n, int n8, int T) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;

@@ -70,11 +70,11 @@ __global__ void __launch_bounds__(256) kda_gate8_kernel(const KdaGateParams p) {
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
   }
   if (p.bias) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p.bias + col));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + col + 4));
+    const float4 a = *reinterpret_cast<const float4*>(p.bias + col);
+    const float4 b = *reinterpret_cast<const float4*>(p.bias + col + 4);
     x[0] += a.x; x[1] += a.y; x[2] += a.z; x[3] += a.w; x[4] += b.x; x[5] += b.y; x[6] += b.z; x[7] += b.w;
   }
-  const float a = -expf(__ldg(p.a_log + col / p.D));
+  const float a = -expf(p.a_log[col / p.D]);
   const float inv_beta = 1.0f / p.beta;
   float y[8];
 #pragma unroll

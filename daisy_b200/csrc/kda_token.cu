@@ -94,7 +94,7 @@ __device__ __forceinline__ void kt_gate_rows(KtGateRows<HW>& rows, const __nv_bf
 #pragma unroll
   for (int k = 0; k < KtGateRows<HW>::N; ++k) {
     const int r = hw + HW * k;
-    if (r < 256) rows.w[k] = __ldg(reinterpret_cast<const uint4*>((r < 128 ? f1 : g1) + ((size_t)h * 128 + (r & 127)) * 128 + 8 * sub));
+    if (r < 256) rows.w[k] = *reinterpret_cast<const uint4*>((r < 128 ? f1 : g1) + ((size_t)h * 128 + (r & 127)) * 128 + 8 * sub);
   }
 }
 template <int HW>
@@ -128,9 +128,9 @@ __device__ __forceinline__ void kt_gates(float* sv, const KtGateRows<HW>& rows, 
   if (r < 256) {
     float x = __bfloat162float(__float2bfloat16_rn(d[0]));
     if (r < 128) {                                    // decay e^g, g = -exp(A) softplus(f + dt_bias) at bf16
-      const float z = x + __ldg(dt_bias + h * 128 + r);
+      const float z = x + dt_bias[h * 128 + r];
       const float sp_ = z > 20.f ? z : log1pf(expf(z));
-      sv[5 * 128 + r] = __expf(__bfloat162float(__float2bfloat16_rn(-expf(__ldg(a_log + h)) * sp_)));
+      sv[5 * 128 + r] = __expf(__bfloat162float(__float2bfloat16_rn(-expf(a_log[h]) * sp_)));
     } else {
       if (g1_bias) x = __bfloat162float(__float2bfloat16_rn(x + __bfloat162float(g1_bias[h * 128 + r - 128])));
       sv[6 * 128 + r - 128] = x;
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(TK_CT, 1) kda_token_kernel(const __grid_consta
     const int m = KdaTokenStream::matrix(t0 + (r >> 4), p.dim, row);
     if (m < 3) {
       cs = *reinterpret_cast<const uint4*>(p.conv_s[m] + ((size_t)b * p.dim + row + (r & 15)) * 4);
-      cw = __ldg(reinterpret_cast<const uint4*>(p.conv_w[m] + (size_t)(row + (r & 15)) * 4));
+      cw = *reinterpret_cast<const uint4*>(p.conv_w[m] + (size_t)(row + (r & 15)) * 4);
     }
   }
   uint32_t swz[4];
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(TK_CT, 1) kda_token_kernel(const __grid_consta
     if (m < 3) {
       __nv_bfloat16* sp = p.conv_s[m] + ((size_t)b * p.dim + row) * 4;
       uint4 s = cs, w = cw;
-      if (!first) { s = *reinterpret_cast<const uint4*>(sp); w = __ldg(reinterpret_cast<const uint4*>(p.conv_w[m] + (size_t)row * 4)); }
+      if (!first) { s = *reinterpret_cast<const uint4*>(sp); w = *reinterpret_cast<const uint4*>(p.conv_w[m] + (size_t)row * 4); }
       float out[2];
       kt_conv(s, w, v, p.conv_b[m] ? p.conv_b[m] + row : nullptr, p.silu, out);
       *reinterpret_cast<uint4*>(sp) = kt_shift(s, v);
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(256, 2) kda_batch_kernel(const __grid_constant
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const uint32_t v = half ? cur2.y : cur2.x;
-      const uint4 s = *reinterpret_cast<const uint4*>(cs + 8 * half), w = __ldg(reinterpret_cast<const uint4*>(p.conv_w[warp] + (size_t)(ch + 2 * half) * 4));
+      const uint4 s = *reinterpret_cast<const uint4*>(cs + 8 * half), w = *reinterpret_cast<const uint4*>(p.conv_w[warp] + (size_t)(ch + 2 * half) * 4);
       float out[2];
       kt_conv(s, w, v, p.conv_b[warp] ? p.conv_b[warp] + ch + 2 * half : nullptr, p.silu, out);
       *reinterpret_cast<uint4*>(cs + 8 * half) = kt_shift(s, v);
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(256, 2) kda_batch_kernel(const __grid_constant
     for (int k = 8 * lane; k < p.dim; k += 256) {
       float a[8], w[8];
       unpack8(*reinterpret_cast<const uint4*>(p.x + b * p.x_sb + k), a);
-      unpack8(__ldg(reinterpret_cast<const uint4*>(p.b_w + (size_t)h * p.dim + k)), w);
+      unpack8(*reinterpret_cast<const uint4*>(p.b_w + (size_t)h * p.dim + k), w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) d = fmaf(a[e], w[e], d);
     }

@@ -269,13 +269,13 @@ qkv_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p) {
       if (!QKV && p.gate && n0 < p.per) {
         // 32 columns at a time, transposed through the staging rows: a lane then has four columns of eight rows, eight lanes 128
         // bytes of a row
-        const float a = -expf(__ldg(p.a_log + (n0 >> 7)));
+        const float a = -expf(p.a_log[n0 >> 7]);
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
           uint32_t r[32];
           tmem_ld32(t0 + 32 * q, r);
           const int c = 4 * (lane & 7);
-          const float4 bias = __ldg(reinterpret_cast<const float4*>(p.dt_bias + n0 + 32 * q + c));
+          const float4 bias = *reinterpret_cast<const float4*>(p.dt_bias + n0 + 32 * q + c);
           tc_wait_ld();
 #pragma unroll
           for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(stg + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
@@ -600,12 +600,12 @@ small_gemm_kernel(const __grid_constant__ GemmMaps maps, const GemmParams p, con
     }
     if (!QKV && p.gate && prod == 0) {
       if (mine) {
-        const float a = -expf(__ldg(p.a_log + (w_lo >> 7)));
+        const float a = -expf(p.a_log[w_lo >> 7]);
         float4* d = reinterpret_cast<float4*>(p.gate + (size_t)m * p.per + w_lo);
         const float4* bp = reinterpret_cast<const float4*>(p.dt_bias + w_lo);
 #pragma unroll
         for (int i = 0; i < BN / 4; ++i) {
-          const float4 bias = __ldg(bp + i);
+          const float4 bias = bp[i];
           const uint64_t bias2[2] = {pack2f(bias.x, bias.y), pack2f(bias.z, bias.w)};
           uint64_t v[2] = {pack2f(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])), pack2f(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]))};
           gemm_decay2(v, bias2, a);

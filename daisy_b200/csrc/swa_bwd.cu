@@ -307,7 +307,7 @@ swa_bwd_kv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           int a = k + 1;
           while (a < c) {
             const int m = (a + c) >> 1;
-            if (__ldg(doc_row + m) > k) c = m; else a = m + 1;
+            if (doc_row[m] > k) c = m; else a = m + 1;
           }
         }
         end[e] = k < T ? c : 0;
@@ -329,7 +329,7 @@ swa_bwd_kv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int q = y * WB + lane + 32 * e;
-          l[e] = q < T ? -__ldg(lse + q) : 0.f; d[e] = q < T ? -__ldg(delta + q) : 0.f;
+          l[e] = q < T ? -lse[q] : 0.f; d[e] = q < T ? -delta[q] : 0.f;
         }
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->c_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag, p.status, 9));
         if (!ok) break;
@@ -958,11 +958,11 @@ __device__ __forceinline__ void prep_grad_rows(const PrepGradParams& p) {
     y[i][0] = ld_stream16(p.y[which] + off); y[i][1] = ld_stream16(p.y[which] + off + 64);
     g[i][0] = ld_stream16(p.gy[which] + off); g[i][1] = ld_stream16(p.gy[which] + off + 64);
     if (which == 2 && p.ve) { e[i][0] = ld_stream16(p.ve + off); e[i][1] = ld_stream16(p.ve + off + 64); }
-    rr[i] = __ldg(p.rstd + ((int64_t)m[i] * 3 + which) * p.H + h[i]);
+    rr[i] = p.rstd[((int64_t)m[i] * 3 + which) * p.H + h[i]];
     if (which < 2) {
       const int64_t t = (int64_t)(m[i] % (uint32_t)p.T) * 64 + 8 * sub;
-      cs[i][0] = __ldg(reinterpret_cast<const float4*>(p.cos + t)); cs[i][1] = __ldg(reinterpret_cast<const float4*>(p.cos + t) + 1);
-      cs[i][2] = __ldg(reinterpret_cast<const float4*>(p.sin + t)); cs[i][3] = __ldg(reinterpret_cast<const float4*>(p.sin + t) + 1);
+      cs[i][0] = *reinterpret_cast<const float4*>(p.cos + t); cs[i][1] = (reinterpret_cast<const float4*>(p.cos + t))[1];
+      cs[i][2] = *reinterpret_cast<const float4*>(p.sin + t); cs[i][3] = (reinterpret_cast<const float4*>(p.sin + t))[1];
     }
   }
   float share = 0.f;

@@ -171,8 +171,8 @@ template <bool F16>
 __device__ __forceinline__ void tk_prepare(const TokenParams& p, const TokenGeom& g, const TokenLayer& ly, TokenBars* bars, uint16_t* qs,
                                            float* kv, int bh, int sg, bool merger, uint32_t tag, int lane) {
   const int b = bh / p.H, h = bh - b * p.H;
-  const float4 cs = __ldg(reinterpret_cast<const float4*>(ly.cos + g.pos * 64) + (lane & 15));
-  const float4 sn = __ldg(reinterpret_cast<const float4*>(ly.sin + g.pos * 64) + (lane & 15));
+  const float4 cs = (reinterpret_cast<const float4*>(ly.cos + g.pos * 64))[lane & 15];
+  const float4 sn = (reinterpret_cast<const float4*>(ly.sin + g.pos * 64))[lane & 15];
   float q[4], k[4], v[4];
   {
     uint4 r[3];
