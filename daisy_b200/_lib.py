@@ -104,7 +104,7 @@ SIGNATURES = {
 class Pages(C.Structure):
     """``daisy_b200_pages``: the pool of a paged cache and its table."""
     _fields_ = [("k", _vp), ("v", _vp), ("p_sb", _i64), ("p_sh", _i64), ("p_sr", _i64), ("table", _vp), ("table_sb", _i64),
-                ("n_pages", _i), ("H", _i), ("page", _i), ("width", _i), ("n_seq", _i)]
+                ("n_pages", _i), ("H", _i), ("page", _i), ("width", _i), ("n_seq", _i), ("max_len", _i)]
 
 _lib = None
 

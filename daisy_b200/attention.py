@@ -427,12 +427,14 @@ class B200CausalSelfAttention(nn.Module):
                       window: Optional[int], cu_seqlens: Optional[Tensor] = None):
         """Prompts, or the next pieces of prompts, of sequences in a paged cache: ``x [n,T,dim]``, or packed ``[1,T_total,dim]`` with
         ``cu_seqlens``; ``table [n, entries]`` their rows of ``cache.table``, ``start`` / ``lens [n]`` (int32 on the device) their
-        tokens in the cache before and with this piece.  Stores the keys and values, returns ``y`` of ``x``'s shape."""
+        tokens in the cache before and with this piece.  Stores the keys and values, returns ``y`` of ``x``'s shape.  A piece that leaves the RoPE
+        table is refused: zeros, and ``ops.check_device_status`` raises."""
         B, T = x.size(0), x.size(1)
         q, k, v = self._project(x)
         kp, vp = cache.layer(layer)
         qp = ops.paged_append(k, v, kp, vp, table, start, self.rotary.cos, self.rotary.sin, cu_seqlens, q, self.norm_eps, QKV_DEFAULT, **self._paged_ve(ve))
-        y = ops.paged_attend(qp, kp, vp, table, lens, window, cu_seqlens, self.attn_scale, bounded_qk=True)      # q, k are RMS-normalised
+        y = ops.paged_attend(qp, kp, vp, table, lens, window, cu_seqlens, self.attn_scale, bounded_qk=True,      # q, k are RMS-normalised
+                             max_len=self.rotary.cos.shape[0])
         return self._linear(y.view(B, T, self.m_dim), self.qkvo_w.detach()[3])
 
     def step_paged(self, x: Tensor, ve: Optional[Tensor], cache: B200PagedKVCache, layer: int, window: Optional[int],

@@ -35,7 +35,8 @@ struct PagedCache {
   const int* table;
   int64_t table_sb;
   int n_pages, H, lg, width, n_seq;  // page = 1 << lg
-  __device__ __forceinline__ int64_t capacity() const { return (int64_t)width << lg; }
+  int cap;                           // positions that the table has, or the caller grants
+  __device__ __forceinline__ int64_t capacity() const { return cap; }
   // byte offset of row `pos` of head h in page `pg`
   __device__ __forceinline__ int64_t at(int pg, int h, int pos) const {
     return 2 * (pg * p_sb + h * p_sh + (pos & ((1 << lg) - 1)) * p_sr);
@@ -64,7 +65,7 @@ namespace daisy_host {
 
 // The cache as the kernels take it, or a status.
 static inline int paged_cache(const daisy_b200_pages* c, int D, daisy::PagedCache* out) {
-  if (!c || !c->k || !c->v || !c->table || c->n_pages <= 0 || c->H <= 0 || c->width <= 0 || c->n_seq <= 0 || c->table_sb < 0) return DAISY_EINVAL;
+  if (!c || !c->k || !c->v || !c->table || c->n_pages <= 0 || c->H <= 0 || c->width <= 0 || c->n_seq <= 0 || c->table_sb < 0 || c->max_len < 0) return DAISY_EINVAL;
   if (D != DAISY_HEAD_DIM) return DAISY_EUNSUPPORTED;
   int lg = 4;
   while (lg < 8 && (1 << lg) != c->page) ++lg;
@@ -73,7 +74,8 @@ static inline int paged_cache(const daisy_b200_pages* c, int D, daisy::PagedCach
   if (!daisy_aligned16(c->k) || !daisy_aligned16(c->v) || ((c->p_sb | c->p_sh | c->p_sr) & 7) || (reinterpret_cast<uintptr_t>(c->table) & 3)) return DAISY_EALIGN;
   // rows are written: none may stand for two
   if (c->p_sr < D || (c->H > 1 && c->p_sh < D) || (c->n_pages > 1 && c->p_sb < D)) return DAISY_EINVAL;
-  *out = daisy::PagedCache{(char*)c->k, (char*)c->v, c->p_sb, c->p_sh, c->p_sr, c->table, c->table_sb, c->n_pages, c->H, lg, c->width, c->n_seq};
+  *out = daisy::PagedCache{(char*)c->k, (char*)c->v, c->p_sb, c->p_sh, c->p_sr, c->table, c->table_sb, c->n_pages, c->H, lg, c->width, c->n_seq, c->width << lg};
+  if (c->max_len > 0 && c->max_len < out->cap) out->cap = c->max_len;
   return DAISY_OK;
 }
 

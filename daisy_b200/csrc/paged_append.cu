@@ -74,6 +74,10 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS, APPEND_BLOCKS) paged_append
   if (first < 0) return;                                             // idle
   if (pos < 0 || pos >= p.c.capacity() || ((p.flags & DAISY_ROPE) && pos >= p.table_rows)) {
     if (p.status && lane == 0) p.status[0] = DAISY_EINVAL;
+    for (int h = h0; h < p.Hq; h += step) {                          // its queries read as zeros: nothing is left undefined
+      uint4* dst = p.q_out + ((int64_t)tok * p.Hq + h) * 16 + sub;
+      dst[0] = dst[8] = make_uint4(0, 0, 0, 0);
+    }
     return;
   }
   const int pg = __ldcg(p.c.table + b * p.c.table_sb + (pos >> p.c.lg));

@@ -936,6 +936,7 @@ daisy_b200_pages pages_of(const Tensor& k, const Tensor& v, const Tensor& table,
   c.table = table.data_ptr<int32_t>(); c.table_sb = table.stride(0);
   c.n_pages = (int)checked_int(k.size(0), "the pool"); c.H = (int)checked_int(k.size(1), "the pool");
   c.page = (int)page; c.width = (int)checked_int(table.size(1), "block_table"); c.n_seq = (int)checked_int(table.size(0), "block_table");
+  c.max_len = 0;
   return c;
 }
 void req_tokens(const Tensor& t, const char* name, int64_t heads, const Tensor& like) {
@@ -1048,9 +1049,11 @@ Tensor paged_decode_step(const Tensor& q, const Tensor& k, const Tensor& v, cons
 }
 
 Tensor paged_attend(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens, int64_t window, const OptTensor& cu, double scale,
-                    const OptTensor& out_, bool bounded) {
+                    const OptTensor& out_, bool bounded, int64_t max_len) {
   bool f16;
-  const daisy_b200_pages c = pages_of(k_pages, v_pages, table, &f16);
+  daisy_b200_pages c = pages_of(k_pages, v_pages, table, &f16);
+  TORCH_CHECK_VALUE(max_len >= 0, "max_len must not be negative, got ", max_len);
+  c.max_len = (int)std::min<int64_t>(max_len, INT32_MAX);
   c10::cuda::CUDAGuard guard(k_pages.device());
   req(q, "q", k_pages.scalar_type());
   TORCH_CHECK_VALUE(q.device() == k_pages.device(), "q is on ", q.device(), ", the pages are on ", k_pages.device());

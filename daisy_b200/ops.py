@@ -427,7 +427,7 @@ def paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlen
     stored.  ``cos, sin`` are whole tables ``[rows, 64]``, indexed by position.
 
     ``q`` (raw, ``Hq`` heads): returned normalised and rotated, in the pages' type, for :func:`paged_attend`; rows of idle
-    sequences and of nobody's tokens are not written.  ``ve`` with ``ve_gate_logit`` mixes the value embedding into the
+    sequences and of nobody's tokens are not written, those of tokens whose position is refused are zero.  ``ve`` with ``ve_gate_logit`` mixes the value embedding into the
     normalised v as in :func:`qkv_prep`.  Positions outside the block table or the RoPE tables and pages outside the pool are
     not stored and show up in :func:`check_device_status`.  The index tensors are read on the device only."""
     return ext().paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlens, q, eps, flags, ve, ve_gate_logit)
@@ -456,16 +456,18 @@ def paged_decode_step(q_new, k_new, v_new, k_pages, v_pages, block_table, lens, 
 
 
 def paged_attend(q, k_pages, v_pages, block_table, lens, window: Optional[int], cu_seqlens: Optional[torch.Tensor] = None,
-                 scale: float = ATTN_SCALE, out: Optional[torch.Tensor] = None, bounded_qk: bool = False):
+                 scale: float = ATTN_SCALE, out: Optional[torch.Tensor] = None, bounded_qk: bool = False, max_len: Optional[int] = None):
     """Causal attention of a chunk of every sequence over a paged cache that holds the chunk's keys and values already
     (:func:`paged_append`, whose returned queries this takes): ``q`` prepared, in the pages' type, ``[n, T, Hq, 128]`` or packed
     ``[1, T_total, Hq, 128]`` with ``cu_seqlens``.  ``lens`` int32 ``[n]`` on the device: tokens of each sequence with its chunk;
     a sequence's queries are its last ones.  Each sees the nearest ``window`` keys up to its own (None: all); cached rows that none of
     them sees may hold anything (an infinity or NaN in a value row that some see may reach the others).  Rows of idle
-    sequences (``lens`` negative) and of sequences that hold fewer tokens than the chunk are zero (the latter show up in
-    :func:`check_device_status`), rows past ``cu_seqlens[n]`` are not written.  ``bounded_qk`` as in :func:`swa_attend`
-    (bf16 pages).  Returns bf16 of ``q``'s shape."""
-    return ext().paged_attend(q, k_pages, v_pages, block_table, lens, int(window or 0), cu_seqlens, scale, out, bounded_qk)
+    sequences (``lens`` negative), of sequences that hold fewer tokens than the chunk and of those longer than the table are zero (the
+    latter two show up in :func:`check_device_status`), rows past ``cu_seqlens[n]`` are not written.  ``bounded_qk`` as in :func:`swa_attend`
+    (bf16 pages).  ``max_len``: tokens a sequence may have, where that is less than the block table has room for (the rows of a RoPE
+    table, behind which the append stores nothing); a longer one is refused like one that the table does not hold.  Returns bf16 of
+    ``q``'s shape."""
+    return ext().paged_attend(q, k_pages, v_pages, block_table, lens, int(window or 0), cu_seqlens, scale, out, bounded_qk, int(max_len or 0))
 
 
 def kda_chunk_fwd(q, k, v, g, beta, scale: Optional[float] = None, initial_state=None,

@@ -555,8 +555,9 @@ int daisy_b200_kda_token_step(const daisy_b200_kda_layer* layer, const void* x, 
  *   table      int32: position p of sequence b lies in row p % page of page table[b * table_sb + p / page]; entries that no
  *              visible or new position needs are not read
  *   page       16, 32, 64, 128 or 256; width entries a sequence
+ *   max_len    positions a sequence may have, 0: as many as the table does (width * page)
  * Index arrays (table, start, lens, cu) are read on the device, so a launch can be captured and replayed while they
- * change.  What they ask for is checked there: a position outside the table's width or the RoPE tables, or a page outside
+ * change.  What they ask for is checked there: a position outside max_len, the table's width or the RoPE tables, or a page outside
  * 0 .. n_pages-1, writes DAISY_EINVAL to the status word; nothing is stored for such a position, a row read from such a
  * page is taken from page 0. */
 typedef struct daisy_b200_pages {
@@ -565,6 +566,7 @@ typedef struct daisy_b200_pages {
   const int32_t* table;
   int64_t table_sb;
   int n_pages, H, page, width, n_seq;
+  int max_len;
 } daisy_b200_pages;
 
 /* Keys and values of new tokens to their pages, RMS-normalised and rotated on the way (flags as daisy_b200_qkv_prep); the
@@ -574,7 +576,8 @@ typedef struct daisy_b200_pages {
  *   start      int32 [n_seq]: position of each sequence's first new token, negative: the sequence is idle
  *   cu         NULL: B = n_seq, sequence b owns the T tokens of row b.  Else B = 1 and int32 [n_seq + 1]: sequence b owns tokens
  *              cu[b] .. cu[b+1]-1 of the T; tokens at or past cu[n_seq] belong to nobody
- *   q_out      [B,T,Hq,D] contiguous, in the pages' type; rows of idle sequences and of nobody's tokens are left as they were
+ *   q_out      [B,T,Hq,D] contiguous, in the pages' type; rows of idle sequences and of nobody's tokens are left as they were,
+ *              of tokens whose position is refused zero
  *   cos, sin   whole tables [table_rows, D/2] float32
  *   ve, ve_gate_logit   as daisy_b200_qkv_prep, logical [B,T,H,D] beside v; NULL: none */
 int daisy_b200_paged_append(const daisy_b200_pages* cache, const void* k, const void* v, const void* q,
@@ -611,11 +614,12 @@ int daisy_b200_paged_decode_step(const daisy_b200_pages* cache, const void* q_ne
  * chunk sees may hold anything; an infinity or NaN in a value row that some of its queries see may reach the others.
  *   q          prepared (q_out of daisy_b200_paged_append), logical [B,T,Hq,D] with strides (s_b,s_t,s_h), of the PAGES' type;
  *              Hq a multiple of the cache's H
- *   lens       int32 [n_seq]: tokens of the sequence with this chunk, negative: idle
+ *   lens       int32 [n_seq]: tokens of the sequence with this chunk, negative: idle.  Where a RoPE table is shorter than the block table, give its
+ *              rows as max_len: the append stores nothing behind them
  *   cu         NULL: B = n_seq, T queries a sequence; else B = 1, int32 [n_seq + 1], as daisy_b200_paged_append (offsets outside 0 .. T or
  *              decreasing are refused)
  *   out        [B,T,Hq,D] bf16, strides (o_sb,o_st,o_sh); rows of idle or refused sequences (fewer tokens than queries, more
- *              than the table holds) are zero, rows of nobody's tokens are left as they were
+ *              than the table holds or than max_len) are zero, rows of nobody's tokens are left as they were
  *   flags      DAISY_BOUNDED_QK as in daisy_b200_swa_attend | DAISY_CACHE_FP16
  *   workspace  daisy_b200_paged_attend_workspace_bytes(B,T,n_seq,Hq,H) bytes on the current device (80 MB and the list of work
  *              items), 256-byte aligned, scratch; calls that may overlap on the device need workspaces of their own

@@ -41,3 +41,57 @@ def test_float16_weights_far_below_the_largest(T):
     assert (2.0 ** -5 * ref > tol).all()
     over = (y.double().cpu() - ref[None, :, None]).abs() - tol[None, :, None]
     assert (over <= 0).all(), f"{over.max().item():.3g} over the tolerance; off by up to {((y.double().cpu() / ref[None, :, None]) - 1).abs().max().item():.3g} of the value"
+
+
+def test_tokens_behind_the_rope_table():
+    """A block table longer than the RoPE table: what is stored stays stored, refused tokens' queries and their sequences' outputs are zero."""
+    from daisy_b200 import _lib, ops
+    H, page, T, rope = 2, 16, 20, 50
+    cos, sin = (t.cuda() for t in _tables(rope))
+    x = _randn(_gen(1), 3, T, 3 * H, D).cuda()
+    table = torch.arange(12).view(3, 4).int().cuda()                 # 64 positions a sequence
+    start = _ints([0, 40, 60])                                       # inside; across the RoPE table's end; across both ends
+    fill = float("nan")
+    k_pages = torch.full((12, H, page, D), fill, dtype=torch.bfloat16, device="cuda")
+    v_pages = k_pages.clone()
+    # the queries' memory comes from the allocator: leave NaN there
+    del_me = torch.full((3, T, H, D), fill, dtype=torch.bfloat16, device="cuda")
+    del del_me
+    q = ops.paged_append(x[:, :, H:2 * H], x[:, :, 2 * H:], k_pages, v_pages, table, start, cos, sin, q=x[:, :, :H], eps=EPS)
+    _status(_lib.EINVAL)
+    assert torch.isfinite(q.float()).all() and (q[1, 10:] == 0).all() and (q[2] == 0).all() and (q[1, :10] != 0).any(-1).all()
+    for T_q in (T, 3):                                               # both kernels
+        y = ops.paged_attend(q[:, -T_q:], k_pages, v_pages, table, start + T, None, bounded_qk=True, max_len=rope)
+        _status(_lib.EINVAL)
+        assert (y[1:] == 0).all() and torch.isfinite(y.float()).all()
+        alone = ops.paged_attend(q[:1, -T_q:], k_pages, v_pages, table[:1], start[:1] + T, None, bounded_qk=True)
+        _status()
+        assert torch.equal(y[:1], alone)
+        # up to the limit and no further
+        assert (ops.paged_attend(q[:1, -T_q:], k_pages, v_pages, table[:1], _ints([T]), None, bounded_qk=True, max_len=T) == alone).all()
+        _status()
+        assert (ops.paged_attend(q[:1, -T_q:], k_pages, v_pages, table[:1], _ints([T]), None, bounded_qk=True, max_len=T - 1) == 0).all()
+        _status(_lib.EINVAL)
+    with pytest.raises(ValueError):
+        ops.paged_attend(q[:1], k_pages, v_pages, table[:1], _ints([T]), None, max_len=-1)
+
+
+def test_layer_prompt_behind_the_rope_table():
+    from daisy_b200 import B200CausalSelfAttention, B200PagedKVCache, _lib
+    H, dim = 2, 256
+    torch.manual_seed(3)
+    a = B200CausalSelfAttention(dim, H, D, max_seq_len=64)
+    with torch.no_grad():
+        a.qkvo_w.copy_(torch.randn(4, dim, dim) * dim ** -0.5)
+    a = a.cuda()
+    assert a.rotary.cos.shape[0] == 64
+    cache = B200PagedKVCache(1, 16, H, D, 2, 128, "cuda", page=16)
+    cache.k.fill_(float("nan"))
+    cache.v.fill_(float("nan"))
+    slots = [cache.claim(), cache.claim()]
+    cache.reserve(slots, 70)
+    x = torch.randn(2, 70, dim, generator=_gen(2)).bfloat16().cuda()
+    with torch.inference_mode():
+        y = a.prefill_paged(x[:, :64], None, cache, 0, cache.table, _ints([0, 6]), _ints([64, 70]), None)
+    _status(_lib.EINVAL)
+    assert torch.isfinite(y.float()).all() and (y[1] == 0).all() and (y[0] != 0).any()
