@@ -780,6 +780,10 @@ extern "C" int daisy_b200_paged_attend_few(const daisy_b200_pages* cache, const 
   if (B != (cu ? 1 : cache->n_seq)) return DAISY_EINVAL;
   const int cols = daisy_b200_paged_attend_few_rows(T, cache->n_seq, cu != nullptr, Hq, cache->H);
   if (cols == 0) return DAISY_EUNSUPPORTED;
+  p.n_grp = (cols + PD_FEW - 1) / PD_FEW;
+  // blocks are counted in 32 bits
+  const int64_t blocks = (int64_t)cache->width * cache->page / (PD_TILE * PD_WARPS) + 2 + PD_HEAD, pairs = (int64_t)cache->n_seq * cache->H * p.n_grp;
+  if (pairs >= (int64_t)1 << 31 || blocks * pairs >= ((int64_t)1 << 31) - 65536) return DAISY_EUNSUPPORTED;
   if (!daisy_aligned16(q) || !daisy_aligned16(workspace) || ((q_sb | q_st | q_sh) & 7) || ((o_sb | o_st | o_sh) & 3) || (reinterpret_cast<uintptr_t>(out) & 7) ||
       (reinterpret_cast<uintptr_t>(lens) & 3) || (reinterpret_cast<uintptr_t>(cu) & 3))
     return DAISY_EALIGN;
@@ -787,9 +791,6 @@ extern "C" int daisy_b200_paged_attend_few(const daisy_b200_pages* cache, const 
   const int sms = daisy_host::sm_count_cached();
   if (sms <= 0) return DAISY_ENODEV;
   p.G = Hq / cache->H; p.Hq = Hq; p.T = T; p.cu = cu;
-  p.n_grp = (cols + PD_FEW - 1) / PD_FEW;
-  const int64_t blocks = (int64_t)cache->width * cache->page / (PD_TILE * PD_WARPS) + 2 + PD_HEAD, pairs = (int64_t)cache->n_seq * cache->H * p.n_grp;
-  if (pairs >= (int64_t)1 << 31 || blocks * pairs >= ((int64_t)1 << 31) - 65536) return DAISY_EUNSUPPORTED;
   p.q = (const __nv_bfloat16*)q; p.q_sb = q_sb; p.q_st = q_st; p.q_sh = q_sh;
   p.out = (__nv_bfloat16*)out; p.o_sb = o_sb; p.o_st = o_st; p.o_sh = o_sh;
   p.lens = lens; p.window = daisy_host::paged_window(cache, window);

@@ -1078,10 +1078,12 @@ Tensor paged_attend(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
   const unsigned flags = (bounded ? DAISY_BOUNDED_QK : 0) | (f16 ? DAISY_CACHE_FP16 : 0);
   if (daisy_b200_paged_attend_few_rows((int)T, c.n_seq, cup != nullptr, (int)checked_int(Hq, "q"), c.H)) {
     const Tensor ws = stream_workspace(q, WS_PAGED_DECODE, (int64_t)daisy_b200_paged_attend_few_workspace_bytes(c.n_seq, c.H, 128));
-    check(daisy_b200_paged_attend_few(&c, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), len, cup, w, out.data_ptr(), out.stride(0), out.stride(1), out.stride(2), (int)B, (int)T,
-                                      (int)Hq, 128, (float)scale, flags, ws.data_ptr(), (size_t)ws.numel(), status_ptr(q), stream_of(q)),
-          "daisy_b200_paged_attend_few");
-    return out;
+    const int rc = daisy_b200_paged_attend_few(&c, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), len, cup, w, out.data_ptr(), out.stride(0), out.stride(1), out.stride(2), (int)B,
+                                               (int)T, (int)Hq, 128, (float)scale, flags, ws.data_ptr(), (size_t)ws.numel(), status_ptr(q), stream_of(q));
+    if (rc != DAISY_EUNSUPPORTED) {                                  // else a table too wide for its count of blocks, which the other form does not have
+      check(rc, "daisy_b200_paged_attend_few");
+      return out;
+    }
   }
   const Tensor ws = at::empty({(int64_t)daisy_b200_paged_attend_workspace_bytes((int)B, (int)T, c.n_seq, (int)checked_int(Hq, "q"), c.H)}, q.options().dtype(at::kByte));
   check(daisy_b200_paged_attend(&c, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), len, cup, w, out.data_ptr(),

@@ -594,6 +594,7 @@ int daisy_b200_paged_append(const daisy_b200_pages* cache, const void* k, const 
  *              of group g read key head g.  k_new, v_new [n_seq,1,H,D]
  *   lens       int32 [n_seq]: tokens in the cache, negative: the sequence is idle (its output is zero, nothing is stored); so
  *              is one whose position is refused
+ *   table      of fewer than 2^31 blocks of 64 positions over all sequences, key heads and passes of 8 (16 where Hq / H > 8) query heads
  *   out        [n_seq,1,Hq,D] bf16 with strides (o_sb,o_sh)
  *   flags      DAISY_QKV_DEFAULT bits | DAISY_CACHE_FP16
  *   workspace  daisy_b200_paged_decode_workspace_bytes(n_seq,Hq,H,D) bytes on the current device, 16-byte aligned, zero
@@ -633,7 +634,8 @@ int daisy_b200_paged_attend(const daisy_b200_pages* cache, const void* q, int64_
 
 /* The same for a few queries of every sequence, split over the cached rows like daisy_b200_paged_decode_step: up to 8 (query, head)
  * pairs of a key head a sequence, or packed rows of up to 32 in all and 4 a sequence on average.
- *   few_rows   T * Hq / H where the call below takes it, 0 where daisy_b200_paged_attend is to
+ *   few_rows   T * Hq / H where the call below takes it, 0 where daisy_b200_paged_attend is to.  The table is not looked at: one of more than 2^31
+ *              blocks of 64 positions over all sequences, key heads and passes of 8 pairs is refused (DAISY_EUNSUPPORTED), and daisy_b200_paged_attend takes it
  *   workspace  daisy_b200_paged_attend_few_workspace_bytes bytes, 16-byte aligned, zero before the first call, afterwards left to
  *              the calls (it may be one workspace with daisy_b200_paged_decode_step) */
 int    daisy_b200_paged_attend_few_rows(int T, int n_seq, int packed, int Hq, int H);

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_paged import D, EPS, SCALE, _attend_tol, _decode_tol, _gen, _ints, _randn, _status, _tables
+from test_gpu_paged import D, EPS, SCALE, _attend_tol, _attention, _check, _decode_tol, _gen, _ints, _randn, _status, _tables
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +95,22 @@ def test_layer_prompt_behind_the_rope_table():
         y = a.prefill_paged(x[:, :64], None, cache, 0, cache.table, _ints([0, 6]), _ints([64, 70]), None)
     _status(_lib.EINVAL)
     assert torch.isfinite(y.float()).all() and (y[1] == 0).all() and (y[0] != 0).any()
+
+
+@pytest.mark.parametrize("T", [3, 40])
+def test_chunks_over_a_very_wide_table(T):
+    """A short chunk over a table with more blocks than the form for few queries counts goes by the other one."""
+    from daisy_b200 import ops
+    n, page, width, lens = 128, 256, 2 ** 22, 300
+    g = _gen(7)
+    k, v = (_randn(g, 2, 1, page, D) for _ in range(2))
+    q = torch.randn(n, T, 1, D, generator=g).bfloat16()
+    row = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+    row[0, :2] = _ints([1, 0])
+    y = ops.paged_attend(q.cuda(), k.cuda(), v.cuda(), row.expand(n, -1), _ints([lens - b for b in range(n)]), None)
+    _status()
+    kk, vv = (x.flip(0)[:, 0].flatten(0, 1)[None].double() for x in (k, v))
+    for b in range(n):
+        seen = torch.arange(2 * page)[None] <= (lens - b - T + torch.arange(T))[:, None]
+        ref, A, mass = _attention(q[b].double(), kk, vv, seen)
+        _check(y[b], ref, _attend_tol(ref, A, mass, lens, torch.bfloat16, 0.0, False), f"sequence {b}")
