@@ -168,7 +168,7 @@ class B200PagedKVCache:
 
     def reserve(self, slots: Iterable[int], tokens) -> None:
         """Pages for ``tokens`` (a number, or one for each slot) more tokens of every sequence; raises ``RuntimeError``, with
-        nothing changed, where the pool has too few."""
+        nothing changed, where the pool has too few (``ValueError`` where a sequence would outgrow its row of the table)."""
         slots = list(slots)
         counts = [tokens] * len(slots) if isinstance(tokens, int) else list(tokens)
         self._store(self.book.reserve(slots, counts))
@@ -178,7 +178,8 @@ class B200PagedKVCache:
         self._store(self.book.forget(slot, before))
 
     def advance(self, slots: Iterable[int], tokens) -> None:
-        """Count ``tokens`` (a number, or one for each slot) stored tokens."""
+        """Count ``tokens`` (a number, or one for each slot) stored tokens; raises ``ValueError``, with nothing changed, where a sequence
+        has no pages for them."""
         slots = list(slots)
         counts = [tokens] * len(slots) if isinstance(tokens, int) else list(tokens)
         self.book.advance(slots, counts)
@@ -218,13 +219,20 @@ class PageBook:
         self.table[slot] = [-1] * len(row)
         self.length[slot], self.first[slot], self.end[slot] = -1, 0, 0
 
-    def reserve(self, slots, counts):
-        want = {}
+    def _tokens(self, slots, counts):
+        """Tokens by slot (one that comes twice has both counts), each with room in the table."""
+        if len(slots) != len(counts):
+            raise ValueError(f"{len(counts)} counts for {len(slots)} slots")
+        tokens = {}
         for slot, n in zip(slots, counts):
             self._check(slot)
-            if n < 0 or self.length[slot] + n > self.max_len:
-                raise ValueError(f"slot {slot}: {self.length[slot]} + {n} tokens, the table holds {self.max_len}")
-            want[slot] = max(want.get(slot, 0), -(-(self.length[slot] + n) // self.page) - self.end[slot])
+            tokens[slot] = tokens.get(slot, 0) + n
+            if n < 0 or self.length[slot] + tokens[slot] > self.max_len:
+                raise ValueError(f"slot {slot}: {self.length[slot]} + {tokens[slot]} tokens, the table holds {self.max_len}")
+        return tokens
+
+    def reserve(self, slots, counts):
+        want = {slot: -(-(self.length[slot] + n) // self.page) - self.end[slot] for slot, n in self._tokens(slots, counts).items()}
         if sum(max(w, 0) for w in want.values()) > len(self.free):
             raise RuntimeError(f"the paged cache has {len(self.free)} pages left")
         changed = [slot for slot, w in want.items() if w > 0]
@@ -246,8 +254,9 @@ class PageBook:
         return [slot]
 
     def advance(self, slots, counts):
-        for slot, n in zip(slots, counts):
-            self._check(slot)
-            if n < 0 or self.length[slot] + n > self.end[slot] * self.page:
+        tokens = self._tokens(slots, counts)
+        for slot, n in tokens.items():
+            if self.length[slot] + n > self.end[slot] * self.page:
                 raise ValueError(f"slot {slot} has no pages for {n} more tokens")
+        for slot, n in tokens.items():
             self.length[slot] += n

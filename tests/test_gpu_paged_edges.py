@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_paged import D, EPS, SCALE, _attend_tol, _attention, _check, _decode_tol, _gen, _ints, _randn, _status, _tables
+from test_gpu_paged import D, EPS, SCALE, _attend_tol, _attention, _check, _decode_tol, _gen, _ints, _randn, _stack, _status, _tables
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +114,43 @@ def test_chunks_over_a_very_wide_table(T):
         seen = torch.arange(2 * page)[None] <= (lens - b - T + torch.arange(T))[:, None]
         ref, A, mass = _attention(q[b].double(), kk, vv, seen)
         _check(y[b], ref, _attend_tol(ref, A, mass, lens, torch.bfloat16, 0.0, False), f"sequence {b}")
+
+
+@pytest.mark.parametrize("window,page", [(None, 16), (90, 32), (33, 64)])
+@pytest.mark.parametrize("graph", [False, True])
+def test_runner_out_of_pages(window, page, graph):
+    """Prompts and steps that the pool has no pages for are refused with nothing changed, and served once a sequence has ended."""
+    from daisy_b200 import PagedRunner
+    H, dim = 1, D
+    runner = PagedRunner(_stack(1, H, dim), window, pages=6, max_seqs=2, max_len=6 * page, page=page)
+    if graph:
+        runner.capture_step(dim)
+    step = runner.step_graph if graph else runner.step
+    c = runner.cache
+    g = _gen(11)
+
+    def prompt(n):
+        return torch.randn(n, dim, generator=g).bfloat16().cuda()
+
+    def state():
+        return list(c.length), [list(r) for r in c.book.table], sorted(c.book.free), c.lens.tolist(), c.table.tolist()
+    a, b = runner.add(), runner.add()
+    runner.prefill([prompt(page), prompt(page)], [a, b])             # full pages: the next token needs one each
+    held = {s: c.book.end[s] - c.book.first[s] for s in (a, b)}
+    assert held == {a: 1, b: 1}
+    before = state()
+    with pytest.raises(RuntimeError, match="4 pages left"):
+        runner.prefill([prompt(4 * page), prompt(1)], [a, b])
+    assert state() == before
+    runner.prefill([prompt(3 * page)], [a])
+    while c.book.free:                                               # (pages behind a window have come back); a's are full
+        c.reserve([b], (c.book.end[b] + 1) * page - c.length[b])
+    before = state()
+    x = torch.randn(2, 1, dim, generator=g).bfloat16().cuda()
+    with pytest.raises(RuntimeError, match="0 pages left"):
+        step(x)
+    assert state() == before
+    runner.drop(b)
+    y = step(x)
+    assert torch.isfinite(y).all() and (y[a] != 0).any() and (y[b] == 0).all() and c.length == [4 * page + 1, -1]
+    _status()

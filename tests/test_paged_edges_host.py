@@ -2,6 +2,7 @@
 import pytest
 
 from daisy_b200 import _lib
+from daisy_b200.kv_cache import PageBook
 from test_paged_host import _append, _attend, _decode, _pages, address, lib      # noqa: F401
 
 
@@ -22,3 +23,36 @@ def test_few_queries_over_a_table_of_too_many_blocks(lib, address, over, call): 
     assert lib.daisy_b200_paged_attend_few_rows(call.get("T", 1), d["n_seq"], int("cu" in call), call.get("Hq", 4), d["H"]) > 0
     got = _attend(lib, address, pages, few=True, **call)
     assert (got == _lib.EUNSUPPORTED) == (blocks >= 2 ** 31)
+
+
+def _state(book):
+    return list(book.length), [list(r) for r in book.table], list(book.free), list(book.first), list(book.end)
+
+
+def test_a_refused_advance_changes_nothing():
+    book = PageBook(6, 3, 40, 16)
+    a, b, c = book.claim(), book.claim(), book.claim()
+    book.reserve([a, b], [33, 40])
+    before = _state(book)
+    for slots, counts, what in (([a, c], [5, 5], "no pages for"), ([a, b], [5, 41], "the table holds 40"), ([b, a], [1, -1], "tokens"), ([a, 3], [1, 1], "holds no sequence"),
+                                ([a, b], [1], "1 counts for 2 slots"), ([b, b], [30, 11], "the table holds 40")):
+        with pytest.raises(ValueError, match=what):
+            book.advance(slots, counts)
+        assert _state(book) == before
+    book.advance([a, b, a], [20, 40, 13])
+    assert book.length == [33, 40, 0]
+
+
+def test_reserve_adds_up_what_one_slot_asks_for():
+    book = PageBook(6, 2, 64, 16)
+    a, b = book.claim(), book.claim()
+    assert book.reserve([a, a], [10, 10]) == [a] and book.end[a] == 2
+    book.advance([a, a], [10, 10])
+    before = _state(book)
+    with pytest.raises(ValueError, match="20 . 50 tokens, the table holds 64"):
+        book.reserve([b, a, a], [1, 25, 25])
+    with pytest.raises(ValueError, match="2 counts for 1 slots"):
+        book.reserve([b], [1, 1])
+    with pytest.raises(RuntimeError, match="4 pages left"):
+        book.reserve([b, a, b], [30, 40, 30])
+    assert _state(book) == before
