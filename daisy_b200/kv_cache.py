@@ -244,7 +244,7 @@ class PageBook:
 
     def forget(self, slot, before):
         self._check(slot)
-        upto = min(max(before, 0) // self.page, self.end[slot])
+        upto = max(min(before, self.length[slot]), 0) // self.page          # pages of tokens that are yet to come stay
         if upto <= self.first[slot]:
             return []
         row = self.table[slot]

@@ -56,3 +56,15 @@ def test_reserve_adds_up_what_one_slot_asks_for():
     with pytest.raises(RuntimeError, match="4 pages left"):
         book.reserve([b, a, b], [30, 40, 30])
     assert _state(book) == before
+
+
+def test_forget_keeps_the_pages_of_tokens_to_come():
+    """Only what is in the cache can be left behind: reserved pages that wait for their tokens stay."""
+    book = PageBook(6, 1, 96, 16)
+    a = book.claim()
+    book.reserve([a], [80])
+    book.advance([a], [33])
+    assert book.forget(a, 1000) == [a] and book.first[a] == 2 and len(book.free) == 3
+    assert all(p >= 0 for p in book.table[a][2:5])
+    book.advance([a], [47])
+    assert book.length[a] == 80
