@@ -723,6 +723,8 @@ extern "C" int daisy_b200_paged_decode_step(const daisy_b200_pages* cache, const
       (reinterpret_cast<uintptr_t>(out) & 7) || ((o_sb | o_sh) & 3))
     return DAISY_EALIGN;
   if ((flags & DAISY_ROPE) && (!daisy_aligned16(cos) || !daisy_aligned16(sin))) return DAISY_EALIGN;
+  // rows are written: none may stand for two
+  if ((cache->n_seq > 1 && o_sb <= 0) || (Hq > 1 && o_sh <= 0)) return DAISY_EINVAL;
   if (workspace_bytes < daisy_b200_paged_decode_workspace_bytes(cache->n_seq, Hq, cache->H, D)) return DAISY_EWORKSPACE;
   const int sms = daisy_host::sm_count_cached();
   if (sms <= 0) return DAISY_ENODEV;
@@ -787,6 +789,8 @@ extern "C" int daisy_b200_paged_attend_few(const daisy_b200_pages* cache, const 
   if (!daisy_aligned16(q) || !daisy_aligned16(workspace) || ((q_sb | q_st | q_sh) & 7) || ((o_sb | o_st | o_sh) & 3) || (reinterpret_cast<uintptr_t>(out) & 7) ||
       (reinterpret_cast<uintptr_t>(lens) & 3) || (reinterpret_cast<uintptr_t>(cu) & 3))
     return DAISY_EALIGN;
+  // rows are written: none may stand for two
+  if ((T > 1 && o_st <= 0) || (Hq > 1 && o_sh <= 0) || (B > 1 && o_sb <= 0)) return DAISY_EINVAL;
   if (workspace_bytes < daisy_b200_paged_attend_few_workspace_bytes(cache->n_seq, cache->H, D)) return DAISY_EWORKSPACE;
   const int sms = daisy_host::sm_count_cached();
   if (sms <= 0) return DAISY_ENODEV;

@@ -1006,6 +1006,11 @@ OptTensor paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, 
   return out;
 }
 
+// A caller's result tensor: rows of their own for every token and head
+void req_rows(const Tensor& out) {
+  for (int64_t d = 0; d < 3; ++d) TORCH_CHECK_VALUE(out.size(d) <= 1 || out.stride(d) > 0, "out is a broadcast view: tokens or heads would share a row");
+}
+
 int64_t paged_decode_workspace_bytes(int64_t n_seq, int64_t Hq, int64_t H) {
   return (int64_t)daisy_b200_paged_decode_workspace_bytes((int)n_seq, (int)Hq, (int)H, 128);
 }
@@ -1032,6 +1037,7 @@ Tensor paged_decode_step(const Tensor& q, const Tensor& k, const Tensor& v, cons
     req(out, "out");
     TORCH_CHECK_VALUE(out.device() == k_pages.device() && out.dim() == 4 && out.size(0) == n && out.size(1) == 1 && out.size(2) == Hq && out.size(3) == 128, "out must be [", n,
                       ", 1, ", Hq, ", 128] on ", k_pages.device());
+    req_rows(out);
   } else {
     out = at::empty({n, 1, Hq, 128}, q.options());
   }
@@ -1069,6 +1075,7 @@ Tensor paged_attend(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
     out = *out_;
     req(out, "out");
     TORCH_CHECK_VALUE(out.device() == q.device() && out.sizes() == q.sizes(), "out must be ", q.sizes(), " on ", q.device());
+    req_rows(out);
   } else {
     out = at::empty({B, T, Hq, 128}, bf16);
   }
@@ -1086,11 +1093,15 @@ Tensor paged_attend(const Tensor& q, const Tensor& k_pages, const Tensor& v_page
     }
   }
   const Tensor ws = at::empty({(int64_t)daisy_b200_paged_attend_workspace_bytes((int)B, (int)T, c.n_seq, (int)checked_int(Hq, "q"), c.H)}, q.options().dtype(at::kByte));
-  check(daisy_b200_paged_attend(&c, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), len, cup, w, out.data_ptr(),
-                                out.stride(0), out.stride(1), out.stride(2), (int)B, (int)T, (int)Hq, 128, (float)scale,
-                                flags, ws.data_ptr(), (size_t)ws.numel(), status_ptr(q),
-                                stream_of(q)),
+  // The tile copies want rows of their own and 16-byte boundaries, which the form for few queries does without: what either takes is taken.
+  // (rows of nobody's tokens are left as they were: the copy begins as what `out` holds)
+  auto broadcast = [](const Tensor& t) { return (t.size(0) > 1 && t.stride(0) == 0) || (t.size(1) > 1 && t.stride(1) == 0) || (t.size(2) > 1 && t.stride(2) == 0); };
+  const Tensor qt = broadcast(q) ? q.contiguous() : q;
+  const Tensor to = on16(out) && !((out.stride(0) | out.stride(1) | out.stride(2)) & 7) ? out : out.clone(at::MemoryFormat::Contiguous);
+  check(daisy_b200_paged_attend(&c, qt.data_ptr(), qt.stride(0), qt.stride(1), qt.stride(2), len, cup, w, to.data_ptr(), to.stride(0), to.stride(1), to.stride(2), (int)B, (int)T,
+                                (int)Hq, 128, (float)scale, flags, ws.data_ptr(), (size_t)ws.numel(), status_ptr(q), stream_of(q)),
         "daisy_b200_paged_attend");
+  if (!to.is_same(out)) out.copy_(to);
   return out;
 }
 

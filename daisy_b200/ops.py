@@ -459,7 +459,7 @@ def paged_attend(q, k_pages, v_pages, block_table, lens, window: Optional[int], 
                  scale: float = ATTN_SCALE, out: Optional[torch.Tensor] = None, bounded_qk: bool = False, max_len: Optional[int] = None):
     """Causal attention of a chunk of every sequence over a paged cache that holds the chunk's keys and values already
     (:func:`paged_append`, whose returned queries this takes): ``q`` prepared, in the pages' type, ``[n, T, Hq, 128]`` or packed
-    ``[1, T_total, Hq, 128]`` with ``cu_seqlens``.  ``lens`` int32 ``[n]`` on the device: tokens of each sequence with its chunk;
+    ``[1, T_total, Hq, 128]`` with ``cu_seqlens``, also a broadcast view; ``out`` of the same shape, any strides that give every row its own place.  ``lens`` int32 ``[n]`` on the device: tokens of each sequence with its chunk;
     a sequence's queries are its last ones.  Each sees the nearest ``window`` keys up to its own (None: all); cached rows that none of
     them sees may hold anything (an infinity or NaN in a value row that some see may reach the others).  Rows of idle
     sequences (``lens`` negative), of sequences that hold fewer tokens than the chunk and of those longer than the table are zero (the

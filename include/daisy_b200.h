@@ -595,7 +595,7 @@ int daisy_b200_paged_append(const daisy_b200_pages* cache, const void* k, const 
  *   lens       int32 [n_seq]: tokens in the cache, negative: the sequence is idle (its output is zero, nothing is stored); so
  *              is one whose position is refused
  *   table      of fewer than 2^31 blocks of 64 positions over all sequences, key heads and passes of 8 (16 where Hq / H > 8) query heads
- *   out        [n_seq,1,Hq,D] bf16 with strides (o_sb,o_sh)
+ *   out        [n_seq,1,Hq,D] bf16 with strides (o_sb,o_sh), a row of its own for each, 8-byte aligned
  *   flags      DAISY_QKV_DEFAULT bits | DAISY_CACHE_FP16
  *   workspace  daisy_b200_paged_decode_workspace_bytes(n_seq,Hq,H,D) bytes on the current device, 16-byte aligned, zero
  *              before the first call, afterwards left to the calls.  Calls that may overlap on the device need workspaces of
@@ -614,12 +614,12 @@ int daisy_b200_paged_decode_step(const daisy_b200_pages* cache, const void* q_ne
  * (window <= 0: all up to its own).  For prompts behind a cached prefix, prompts in pieces, drafted tokens.  Rows that no query of the
  * chunk sees may hold anything; an infinity or NaN in a value row that some of its queries see may reach the others.
  *   q          prepared (q_out of daisy_b200_paged_append), logical [B,T,Hq,D] with strides (s_b,s_t,s_h), of the PAGES' type;
- *              Hq a multiple of the cache's H
+ *              Hq a multiple of the cache's H; no stride of a dimension longer than 1 may be zero
  *   lens       int32 [n_seq]: tokens of the sequence with this chunk, negative: idle.  Where a RoPE table is shorter than the block table, give its
  *              rows as max_len: the append stores nothing behind them
  *   cu         NULL: B = n_seq, T queries a sequence; else B = 1, int32 [n_seq + 1], as daisy_b200_paged_append (offsets outside 0 .. T or
  *              decreasing are refused)
- *   out        [B,T,Hq,D] bf16, strides (o_sb,o_st,o_sh); rows of idle or refused sequences (fewer tokens than queries, more
+ *   out        [B,T,Hq,D] bf16, strides (o_sb,o_st,o_sh), a row of its own for each, 16-byte aligned; rows of idle or refused sequences (fewer tokens than queries, more
  *              than the table holds or than max_len) are zero, rows of nobody's tokens are left as they were
  *   flags      DAISY_BOUNDED_QK as in daisy_b200_swa_attend | DAISY_CACHE_FP16
  *   workspace  daisy_b200_paged_attend_workspace_bytes(B,T,n_seq,Hq,H) bytes on the current device (80 MB and the list of work
@@ -634,6 +634,7 @@ int daisy_b200_paged_attend(const daisy_b200_pages* cache, const void* q, int64_
 
 /* The same for a few queries of every sequence, split over the cached rows like daisy_b200_paged_decode_step: up to 8 (query, head)
  * pairs of a key head a sequence, or packed rows of up to 32 in all and 4 a sequence on average.
+ *   q          may be a broadcast view (zero strides); out may be 8-byte aligned
  *   few_rows   T * Hq / H where the call below takes it, 0 where daisy_b200_paged_attend is to.  The table is not looked at: one of more than 2^31
  *              blocks of 64 positions over all sequences, key heads and passes of 8 pairs is refused (DAISY_EUNSUPPORTED), and daisy_b200_paged_attend takes it
  *   workspace  daisy_b200_paged_attend_few_workspace_bytes bytes, 16-byte aligned, zero before the first call, afterwards left to

@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from test_gpu_paged import D, EPS, SCALE, _attend_tol, _attention, _check, _decode_tol, _gen, _ints, _randn, _stack, _status, _tables
+from test_gpu_paged import (D, EPS, SCALE, Pool, _attend_tol, _attention, _check, _decode_tol, _gen, _ints, _randn, _stack, _status,
+                            _tables)
 
 pytestmark = pytest.mark.gpu
 
@@ -153,4 +154,38 @@ def test_runner_out_of_pages(window, page, graph):
     runner.drop(b)
     y = step(x)
     assert torch.isfinite(y).all() and (y[a] != 0).any() and (y[b] == 0).all() and c.length == [4 * page + 1, -1]
+    _status()
+
+
+@pytest.mark.parametrize("T", [8, 9, 40])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_queries_and_outputs_are_taken_whatever_a_chunk_goes_by(T, dtype):
+    """Broadcast queries and results on 8-byte boundaries: of chunks for either kernel (8 and 9 are the border), with the bits of a plain call."""
+    from daisy_b200 import ops
+    n, H, page, N = 3, 2, 32, 2 * T
+    pool = Pool([70, 100, 64], [0] * n, H, page, dtype, seed=201)
+    k_pages, v_pages, table = pool.gpu()
+    lens = _ints([70, 100, 64])
+    q = (torch.randn(n, T, H, D, generator=_gen(202)) / 3).to(dtype).cuda()
+    for view in (q[:1].expand(n, -1, -1, -1), q[:, :1].expand(-1, T, -1, -1), q[:, :, :1].expand(-1, -1, H, -1)):
+        plain = ops.paged_attend(view.contiguous(), k_pages, v_pages, table, lens, 50)
+        assert torch.equal(ops.paged_attend(view, k_pages, v_pages, table, lens, 50), plain)
+    for at in (0, 4):                                                # rows 264 bytes apart, from a 16-byte boundary and from an 8-byte one
+        wide = torch.full((n, T, H, D + 4), 3.0, dtype=torch.bfloat16, device="cuda")
+        out = wide[..., at:at + D]
+        assert ops.paged_attend(view, k_pages, v_pages, table, lens, 50, out=out).data_ptr() == out.data_ptr()
+        assert torch.equal(out, plain) and (wide[..., D:] == 3.0 if at == 0 else wide[..., :4] == 3.0).all()
+    # packed, with tokens of nobody behind: their rows stay
+    packed, cu = q.flatten(0, 1)[None, :N + 3], _ints([0, T, N, N])
+    plain = ops.paged_attend(packed, k_pages, v_pages, table, lens, 50, cu_seqlens=cu, out=torch.full_like(packed, 9.0, dtype=torch.bfloat16))
+    out = torch.full((1, N + 3, H, D + 4), 9.0, dtype=torch.bfloat16, device="cuda")[..., 4:]
+    ops.paged_attend(packed, k_pages, v_pages, table, lens, 50, cu_seqlens=cu, out=out)
+    assert torch.equal(out, plain) and (out[:, N:] == 9.0).all()
+    for shared in (torch.empty(1, T, H, D), torch.empty(n, 1, H, D), torch.empty(n, T, 1, D)):
+        with pytest.raises(ValueError, match="broadcast"):
+            ops.paged_attend(q, k_pages, v_pages, table, lens, 50, out=shared.bfloat16().cuda().expand(n, T, H, D))
+    x = _randn(_gen(203), n, 1, 3 * H, D).cuda().split(H, 2)
+    for shared in (torch.empty(1, 1, H, D), torch.empty(n, 1, 1, D)):
+        with pytest.raises(ValueError, match="broadcast"):
+            ops.paged_decode_step(*x, k_pages, v_pages, table, lens, None, None, None, flags=0, out=shared.bfloat16().cuda().expand(n, 1, H, D))
     _status()

@@ -68,3 +68,11 @@ def test_forget_keeps_the_pages_of_tokens_to_come():
     assert all(p >= 0 for p in book.table[a][2:5])
     book.advance([a], [47])
     assert book.length[a] == 80
+
+
+def test_results_that_share_rows_are_refused(lib, address):                      # noqa: F811
+    for few in (False, True):
+        for os in ((0, 512, 128), (512 * 4, 0, 128), (512 * 4, 512, 0)):
+            assert _attend(lib, address, _pages(address), few=few, T=4, os=os) == _lib.EINVAL
+    for os in ((0, 128), (512, 0)):
+        assert _decode(lib, address, _pages(address), os=os) == _lib.EINVAL
