@@ -95,7 +95,7 @@ class StepRunner:
         torch.cuda.current_stream(dev).wait_stream(side)
         self.cache.t_dev.copy_(t_saved)                            # the warm-up advanced the device counter
         self._graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self._graph):
+        with torch.cuda.graph(self._graph, stream=side):             # (without one: on a stream of the current device)
             self._gy = self._graph_body()
         self.cache.t_dev.copy_(t_saved)
 
@@ -233,7 +233,7 @@ class PagedRunner:
             body()
         torch.cuda.current_stream(c.device).wait_stream(side)
         self._graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self._graph):
+        with torch.cuda.graph(self._graph, stream=side):             # (without one: on a stream of the current device)
             self._gy = body()
 
     @torch.inference_mode()

@@ -323,7 +323,7 @@ class B200KimiLinearSelfAttention(torch.nn.Module):
             return
         self._graph = torch.cuda.CUDAGraph()
         self._gstates = (self._recurrent_state, *(self._conv_state or ()))     # what the graph updates: kept as long as it is
-        with torch.cuda.graph(self._graph):
+        with torch.cuda.graph(self._graph, stream=side):             # (without one: on a stream of the current device)
             self._gy = self._forward_core(self._gx, None, None, None, use_cache=True)
         restore()
 
