@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from gpu_util import assert_close_bf16
 from test_gpu_paged import (D, EPS, SCALE, Pool, _attend_tol, _attention, _check, _decode_tol, _gen, _ints, _randn, _stack, _status,
                             _tables)
 
@@ -189,3 +190,82 @@ def test_queries_and_outputs_are_taken_whatever_a_chunk_goes_by(T, dtype):
         with pytest.raises(ValueError, match="broadcast"):
             ops.paged_decode_step(*x, k_pages, v_pages, table, lens, None, None, None, flags=0, out=shared.bfloat16().cuda().expand(n, 1, H, D))
     _status()
+
+
+def _laid_out(pool, layout):
+    """The same pool with other strides: rows of all heads together, heads outermost, or gaps between rows, heads and pages."""
+    n, H, page, _ = pool.shape
+    if layout == "rows first":
+        return pool.transpose(1, 2).contiguous().transpose(1, 2)
+    if layout == "heads outermost":
+        return pool.transpose(0, 1).contiguous().transpose(0, 1)
+    big = torch.full((n, H + 1, page + 1, D + 16), 7.0, dtype=pool.dtype, device="cuda")
+    view = big[:, :H, :page, 8:8 + D]
+    view.copy_(pool)
+    return view
+
+
+@pytest.mark.parametrize("layout", ["rows first", "heads outermost", "gaps"])
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_pools_of_any_strides(layout, page, dtype):
+    """Every call over a pool laid out otherwise has the bits of the same call over the contiguous one, in the results and in the pages."""
+    from daisy_b200 import ops
+    H, G, lens, T = 3, 2, [300, 0, 77, 530], 90
+    pool = Pool(lens, [T + 1] * 4, H, page, dtype, seed=211)
+    x = _randn(_gen(212), 4, T, (G + 2) * H, D).cuda()
+    one = _randn(_gen(213), 4, 1, (G + 2) * H, D).cuda()
+    cos, sin = (t.cuda() for t in _tables())
+    got = []
+    for relaid in (False, True):
+        k, v, table = pool.gpu()
+        if relaid:
+            k, v = _laid_out(k, layout), _laid_out(v, layout)
+            assert not k.is_contiguous()
+        q = ops.paged_append(x[:, :, G * H:(G + 1) * H], x[:, :, (G + 1) * H:], k, v, table, _ints(lens), cos, sin, q=x[:, :, :G * H], eps=EPS)
+        after = _ints([n + T for n in lens])
+        res = [q]
+        for window in (None, 100):
+            for bounded in (True, False):
+                res.append(ops.paged_attend(q, k, v, table, after, window, bounded_qk=bounded))
+                res.append(ops.paged_attend(q[:, -3:], k, v, table, after, window, bounded_qk=bounded))
+        res.append(ops.paged_decode_step(one[:, :, :G * H], one[:, :, G * H:(G + 1) * H], one[:, :, (G + 1) * H:], k, v, table, after, 100, cos, sin, eps=EPS))
+        got.append(res + [k.contiguous().view(torch.int16), v.contiguous().view(torch.int16)])
+    _status()
+    for i, (a, b) in enumerate(zip(*got)):
+        assert torch.isfinite(a.float()).all() and torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("window,page", [(None, 32), (70, 16)])
+@pytest.mark.parametrize("graph", [False, True])
+def test_runner_over_float16_pages(window, page, graph):
+    """Prompts in pieces and steps through two layers against the dense layers (whose keys and values are bf16, rounded more coarsely)."""
+    from daisy_b200 import PagedRunner, WindowMask
+    H, L = 2, 2
+    dim = H * D
+    layers = _stack(L, H, dim)
+    runner = PagedRunner(layers, window, pages=40, max_seqs=2, max_len=400, page=page, dtype=torch.float16)
+    assert runner.cache.k.dtype == torch.float16
+    if graph:
+        runner.capture_step(dim)
+    g = _gen(221)
+    a, b = runner.add(), runner.add()
+    fed, got = {a: [], b: []}, {a: [], b: []}
+    for counts in ([150, 7], [3, 40], [60, 129]):                    # both kernels
+        xs = [torch.randn(n, dim, generator=g).bfloat16().cuda() for n in counts]
+        for s, x, y in zip((a, b), xs, runner.prefill(xs, [a, b])):
+            fed[s].append(x)
+            got[s].append(y.clone())
+    for _ in range(20):
+        x = torch.randn(2, 1, dim, generator=g).bfloat16().cuda()
+        y = (runner.step_graph if graph else runner.step)(x)
+        for s in (a, b):
+            fed[s].append(x[s])
+            got[s].append(y[s].clone())
+    _status()
+    for s in (a, b):
+        x = torch.cat(fed[s])[None]
+        for layer in layers:
+            with torch.inference_mode():
+                x, _, _ = layer.prefill(x, None, attn_mask=WindowMask(window))
+        assert_close_bf16(torch.cat(got[s]), x[0], f"sequence {s}")
