@@ -139,7 +139,7 @@ class StepRunner:
 
 class PagedRunner:
     """A stack of attention layers serving up to ``max_seqs`` sequences of uneven length over a paged cache: prompts (whole or in
-    pieces) of several sequences at a time, then one token of every sequence a step.  Pages that ``window`` has left are given back."""
+    pieces) of several sequences at a time, then one token of every sequence a step.  Pages that ``window`` has left are given back.  Layers without value embeddings."""
 
     def __init__(self, layers: Sequence[B200CausalSelfAttention], window: Optional[int], pages: int, max_seqs: int, max_len: int, page: int = 64,
                  device="cuda", dtype=torch.bfloat16):

@@ -123,7 +123,8 @@ class B200PagedKVCache:
     Storage ``k, v [L, pages, H, page, D]``; position ``p`` of the sequence in slot ``s`` lies in row ``p % page`` of page
     ``table[s, p // page]`` (int32, -1: none).  ``lens [max_seqs]`` (int32 on the device, mirrored in ``length``) counts the
     tokens in the cache, -1 marks a free slot.  The kernels (``ops.paged_append``, ``paged_decode_step``, ``paged_attend``) read both on
-    the device; the page bookkeeping is host arithmetic, with a copy to the device only where a row of the table changes."""
+    the device; the page bookkeeping is host arithmetic, with a copy to the device only where a row of the table changes.
+    Lengths only grow: a caller that may reject stored tokens (drafts) keeps lengths and table itself."""
 
     def __init__(self, L, pages, H, D, max_seqs, max_len, device, dtype=torch.bfloat16, page=64):
         dev = torch.device(device)

@@ -449,7 +449,9 @@ def paged_decode_step(q_new, k_new, v_new, k_pages, v_pages, block_table, lens, 
     afterwards.  Sees the nearest ``min(lens, window - 1)`` cached rows and its own row, which is stored to its page.  Idle
     sequences (``lens`` negative) and refused positions give zeros and store nothing.  ``workspace``: from
     :func:`paged_decode_workspace`, for callers that keep one (a captured graph that is replayed beside other calls);
-    otherwise one is kept per stream.  Nothing depends on host values, so a captured call serves every step.  Returns
+    otherwise one is kept per stream.  ``lens`` must not change while the call runs (advance it on the call's stream): the workspace's counts
+    would stay wrong for the calls after it, until it is zeroed (:func:`release_workspaces` for the kept ones).  Nothing depends on host
+    values, so a captured call serves every step.  Returns
     ``y [n,1,Hq,128]`` bf16."""
     return ext().paged_decode_step(q_new, k_new, v_new, k_pages, v_pages, block_table, lens, int(window or 0), cos, sin, scale, eps, flags,
                                    out, workspace, ve, ve_gate_logit)
@@ -459,8 +461,9 @@ def paged_attend(q, k_pages, v_pages, block_table, lens, window: Optional[int], 
                  scale: float = ATTN_SCALE, out: Optional[torch.Tensor] = None, bounded_qk: bool = False, max_len: Optional[int] = None):
     """Causal attention of a chunk of every sequence over a paged cache that holds the chunk's keys and values already
     (:func:`paged_append`, whose returned queries this takes): ``q`` prepared, in the pages' type, ``[n, T, Hq, 128]`` or packed
-    ``[1, T_total, Hq, 128]`` with ``cu_seqlens``, also a broadcast view; ``out`` of the same shape, any strides that give every row its own place.  ``lens`` int32 ``[n]`` on the device: tokens of each sequence with its chunk;
-    a sequence's queries are its last ones.  Each sees the nearest ``window`` keys up to its own (None: all); cached rows that none of
+    ``[1, T_total, Hq, 128]`` with ``cu_seqlens``, also a broadcast view; ``out`` of the same shape, any strides that give every row its own
+    place.  ``lens`` int32 ``[n]`` on the device: tokens of each sequence with its chunk;
+    a sequence's queries are its last ones (neither may change while the call runs, see :func:`paged_decode_step`).  Each sees the nearest ``window`` keys up to its own (None: all); cached rows that none of
     them sees may hold anything (an infinity or NaN in a value row that some see may reach the others).  Rows of idle
     sequences (``lens`` negative), of sequences that hold fewer tokens than the chunk and of those longer than the table are zero (the
     latter two show up in :func:`check_device_status`), rows past ``cu_seqlens[n]`` are not written.  ``bounded_qk`` as in :func:`swa_attend`

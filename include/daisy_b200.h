@@ -599,7 +599,9 @@ int daisy_b200_paged_append(const daisy_b200_pages* cache, const void* k, const 
  *   flags      DAISY_QKV_DEFAULT bits | DAISY_CACHE_FP16
  *   workspace  daisy_b200_paged_decode_workspace_bytes(n_seq,Hq,H,D) bytes on the current device, 16-byte aligned, zero
  *              before the first call, afterwards left to the calls.  Calls that may overlap on the device need workspaces of
- *              their own. */
+ *              their own.  lens must not change while a call runs (nor lens, cu under daisy_b200_paged_attend_few): CTAs that
+ *              deal the work out by different lengths leave counts in the workspace that the calls after them take for their
+ *              own.  After such a call, zero it. */
 size_t daisy_b200_paged_decode_workspace_bytes(int n_seq, int Hq, int H, int D);
 int daisy_b200_paged_decode_step(const daisy_b200_pages* cache, const void* q_new, const void* k_new, const void* v_new,
                                  int64_t q_sb, int64_t q_sh, int64_t k_sb, int64_t k_sh, int64_t v_sb, int64_t v_sh,
