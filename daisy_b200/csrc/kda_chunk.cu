@@ -745,8 +745,6 @@ __global__ void __launch_bounds__(KS_THREADS, 1) kda_state_kernel(const KdaState
       uint32_t u0[16];
 #pragma unroll
       for (int j = 0; j < 4; ++j) ld_shared16(u0 + 4 * j, rec + KS_AU + rec_off(v, 32 * half + 8 * j));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->a_empty[s]);
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->u, c & 1, abort_flag, p.status, 8));
       if (!ok) break;
       tc_fence_after();
@@ -761,6 +759,11 @@ __global__ void __launch_bounds__(KS_THREADS, 1) kda_state_kernel(const KdaState
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(&bars->u16);
+      // Part A is given back when what was loaded from it has been used (the U products give it back too): given back right after the loads,
+      // these were seen to read the copy of three chunks later, once in 20,000 calls or more, beside the intra-chunk pass with L2 cold
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->a_empty[s]);
     }
     if (ok && p.hT) {
       float* hp = p.hT + bh * p.ld_out + 64 * half * KD + v;
