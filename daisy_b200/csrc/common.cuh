@@ -82,6 +82,12 @@ __device__ __forceinline__ void mbar_init_fence() { asm volatile("fence.mbarrier
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// A warp gives shared memory back to the one who writes it next, when the values it has loaded from there are in its registers: an arrive by
+// itself does not wait for loads in flight.  `loaded`: any function of all of them.
+__device__ __forceinline__ void mbar_give_back(uint64_t* bar, int loaded) {
+  const int lane = __any_sync(0xffffffffu, loaded == (int)0x80000001) ? 1 : 0;      // one lane or another
+  if ((threadIdx.x & 31) == lane) mbar_arrive(bar);
+}
 __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }

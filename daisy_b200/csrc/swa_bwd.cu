@@ -177,8 +177,7 @@ swa_bwd_kv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const uint32_t s = it % KV_NI;
     if (!__all_sync(0xffffffffu, mbar_wait(&bars->i_full[s], (it / KV_NI) & 1, abort_flag, p.status, 10))) return false;
     item = bars->item[s];
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&bars->i_empty[s]);
+    mbar_give_back(&bars->i_empty[s], item.x ^ item.y ^ item.z ^ item.w);
     return item.x >= 0;
   };
 
@@ -358,8 +357,7 @@ swa_bwd_kv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->e_full, it & 1, abort_flag, p.status, 6));
       if (!ok) break;
       const int end = ends[row], first_end = ends[0];                 // ends do not decrease with the key
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->e_empty);
+      mbar_give_back(&bars->e_empty, end ^ first_end);
       for (int y = lo; y <= hi; ++y, ++n) {
         const float* cf = col_f + (n & 1) * 2 * WB + 32 * grp;
         const int y0 = y * WB;
