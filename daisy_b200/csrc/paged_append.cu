@@ -22,8 +22,8 @@ struct AppendParams {
   bool streams;                      // more is written than L2 keeps
 };
 
-// Rows that a group of eight lanes keeps in flight, warps a block, blocks a SM.  8 x 8192 tokens, 48 rows a token: 271 us (5.9 TB/s; 4
-// rows, blocks of 8 warps, 2 a SM 303 with plain stores), 3765 packed tokens 22.6 us (28.0 with blocks of 8 warps, 3 a SM: two uneven
+// Rows that a group of eight lanes keeps in flight, warps a block, blocks a SM.  8 x 8192 tokens, 48 rows a token: 272-293 us from card to card
+// (5.5-5.9 TB/s; 4 rows, blocks of 8 warps, 2 a SM took a tenth more), 3765 packed tokens 22-24.5 us (a quarter more with blocks of 8 warps, 3 a SM: two uneven
 // waves), 64 single tokens 2.6 us, launch and the chain of four loads.
 constexpr int APPEND_ROWS = 2;
 constexpr int APPEND_WARPS = 2;
@@ -179,7 +179,7 @@ extern "C" int daisy_b200_paged_append(const daisy_b200_pages* cache, const void
   if (tokens * per_tok >= ((int64_t)1 << 31) - 512) return DAISY_EUNSUPPORTED;
   const int sms = daisy_host::sm_count_cached();
   if (sms <= 0) return DAISY_ENODEV;
-  // warps a token: as many as come nearest to one wave of the SMs (3765 tokens x 48 rows: 20.8 us with one, 0.8 of a wave, 21.9 with two), up to
+  // warps a token: as many as come nearest to one wave of the SMs (3765 tokens x 48 rows: one, 0.8 of a wave, takes 5 % less than two), up to
   // a row for every group of eight lanes where tokens are few
   int64_t split = std::max<int64_t>(((int64_t)sms * APPEND_BLOCKS * APPEND_WARPS + tokens / 2) / tokens, 1);
   if (split > (per_tok + 3) / 4) split = (per_tok + 3) / 4;

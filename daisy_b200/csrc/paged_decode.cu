@@ -1,8 +1,8 @@
 // One new token of every sequence against a paged cache: the work of a batch of uneven lengths dealt out in equal shares, one launch.
 //
-// Bound by HBM: 512 bytes for every cached row and key head, read once for all query heads of the group (64 sequences x 4096 rows x 16
-// heads 321 us, 6.7 TB/s; 1 x 131071 x 16 167 us; 24 of up to 16384 rows, 32 query heads over 8, 135 us; 1 x 511 rows x 6 8.4 us, four
-// of them the chain length -> page -> rows and the join).  The cached rows
+// Bound by HBM: 512 bytes for every cached row and key head, read once for all query heads of the group (from card to card 64 sequences x 4096
+// rows x 16 heads 319-350 us, 6.1-6.7 TB/s, the least where the same rows are read again and L2 still holds some; 1 x 131071 x 16 164-177; 24 of
+// up to 16384 rows, 32 query heads over 8, 133-144; 1 x 511 rows x 6 8.7-9.2, four of them the chain length -> page -> rows and the join).  The cached rows
 // of all (sequence, key head) pairs lie end to end in blocks of four 16-row tiles; every CTA takes an equal run of blocks, whatever sequences it
 // cuts, so neither uneven lengths nor a wide block table leaves an SM idle (the host knows no lengths).  A pair that
 // several CTAs share is joined by the last of them, from partial sums in a fixed order: the same bits every run.  That last one,

@@ -85,7 +85,7 @@ __device__ __forceinline__ int last_tile(int pos, int n) { return (pos + n - 1) 
 // (its sums are written, and read again by the last: 8192 tokens x 16 heads cut in halves 266 us, whole 233).  Whole items take no less than k of
 // the (k - 1) CTAs + 1st longest: of so many, one CTA has k.  The last candidate cuts only
 // the shortest items, as many as whole rounds of all CTAs leave over, into as many pieces as find a CTA then (8192 queries x 16 heads over 65536
-// keys, 512 items: 3700 us whole, 3400 so; three sequences of up to 1500 queries behind up to 9000, whose items make no rounds: 141 and 152).
+// keys, 512 items: in turn on one card 3480 us whole, 3175 so; three sequences of up to 1500 queries behind up to 9000, whose items make no rounds: 141 and 152).
 constexpr float PLAN_COST = 6.f;
 constexpr int PLAN_THREADS = 1024, PLAN_CAND = 6, PLAN_BUCKETS = 1024, PLAN_KEPT = 1024, PLAN_TAIL = 256;
 struct PlanItem { int b, i0, j0, j1, pos, n, row0, cut; };          // j1 < j0: queries that see nothing
@@ -438,7 +438,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       if (g.jhi >= g.jlo) { from = (g.jlo * PP_BN) >> p.c.lg; cur = entries(from); ahead = entries(from + 32); }
       bool next_out = false;
       // The next item is drawn two tiles before this one's last: what is drawn at the start goes to a CTA that may be the last to come to it (8192
-      // queries x 16 heads over 65536 keys 3700 -> 3400 us)
+      // queries x 16 heads over 65536 keys, in turn on one card: 3208 us drawn at the start, 3175 so; 32 over 8 heads, 4096 behind 8000: 564, 552)
       if (g.jhi < g.jlo) draw();
       for (int j = g.jlo; j <= g.jhi && ok; ++j) {
         if (j == max(g.jlo, g.jhi - 2)) draw();
