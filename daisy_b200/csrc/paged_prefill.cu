@@ -497,8 +497,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     const PagedItem* item;
     for (int rd = 0; ok && (item = next_item(rd)); ++rd) {
       const PagedItem g = *item;
-      item_done(rd);
-      if (g.jhi < g.jlo) continue;
+      if (g.jhi < g.jlo) { item_done(rd); continue; }
       for (int j = g.jlo; j <= g.jhi + 1 && ok; ++j) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -558,6 +557,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         }
       }
       n_base += 2 * (g.jhi - g.jlo + 1);
+      item_done(rd);                                                 // not before what was loaded from it has been used
     }
   } else {
     // ------------------------------------------------------------------ softmax + epilogue

@@ -269,3 +269,41 @@ def test_runner_over_float16_pages(window, page, graph):
             with torch.inference_mode():
                 x, _, _ = layer.prefill(x, None, attn_mask=WindowMask(window))
         assert_close_bf16(torch.cat(got[s]), x[0], f"sequence {s}")
+
+
+def test_limits_of_the_library_calls():
+    """``max_len`` of the C interface: positions at or behind it are refused by every call."""
+    import ctypes as C
+    from daisy_b200 import _lib
+    lib, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    H, page, n = 2, 16, 3
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    x = _randn(_gen(241), n, 1, 3 * H, D).cuda()
+    table = torch.arange(12).view(n, 4).int().cuda()
+
+    def pool(limit):
+        k = torch.full((12, H, page, D), float("nan"), dtype=torch.bfloat16, device="cuda")
+        v = k.clone()
+        return k, v, _lib.Pages(k=k.data_ptr(), v=v.data_ptr(), p_sb=H * page * D, p_sh=page * D, p_sr=D, table=table.data_ptr(), table_sb=4, n_pages=12, H=H, page=page, width=4, n_seq=n,
+                                max_len=limit)
+
+    def raised():
+        was = status.item()
+        status.zero_()
+        return was
+    s = 3 * H * D
+    for limit, stored in ((0, 3), (64, 3), (1000, 3), (41, 3), (40, 2), (1, 0)):
+        start = _ints([30, 40, 1])
+        k, v, pages = pool(limit)
+        _lib.check(lib.daisy_b200_paged_append(C.byref(pages), x[:, :, H:].data_ptr(), x[:, :, 2 * H:].data_ptr(), None, s, s, D, s, s, D, 0, 0, 0, None, start.data_ptr(), None, None, None, 0,
+                                               None, 0, 0, 0, None, n, 1, 0, D, EPS, 0, status.data_ptr(), stream), "append")
+        kept = [bool(torch.isfinite(k[b * 4 + p // page, :, p % page].float()).all()) for b, p in enumerate((30, 40, 1))]
+        assert sum(kept) == stored and int(torch.isfinite(k.float()).all(-1).sum()) == stored * H and (raised() != 0) == (stored < 3)
+        k, v, pages = pool(limit)
+        k.zero_(), v.fill_(1.0)
+        ws = torch.zeros(lib.daisy_b200_paged_decode_workspace_bytes(n, H, H, D), dtype=torch.uint8, device="cuda")
+        out = torch.full((n, 1, H, D), 7.0, dtype=torch.bfloat16, device="cuda")
+        _lib.check(lib.daisy_b200_paged_decode_step(C.byref(pages), x.data_ptr(), x[:, :, H:].data_ptr(), x[:, :, 2 * H:].data_ptr(), s, D, s, D, s, D, start.data_ptr(), 0, None, None, 0,
+                                                    out.data_ptr(), H * D, D, None, 0, 0, None, H, D, SCALE, EPS, 0, ws.data_ptr(), ws.numel(), status.data_ptr(), stream), "decode")
+        assert [bool((out[b] != 0).any()) for b in range(n)] == kept and torch.isfinite(out.float()).all() and (raised() != 0) == (stored < 3)
+        assert [bool((v[b * 4 + p // page, :, p % page] != 1).any()) for b, p in enumerate((30, 40, 1))] == kept
